@@ -23,6 +23,23 @@ class MoeWeights(C.Structure):
             "sh_gate_suh", "sh_gate_svh", "sh_up_suh", "sh_up_svh", "sh_down_suh", "sh_down_svh")]
 
 
+class MoeRouting(C.Structure):
+    """``berth_moe_routing`` of include/berth_b200.h."""
+    _fields_ = [("score", _i), ("n_group", _i), ("topk_group", _i), ("group_score", _i), ("renormalize", _i), ("scale", _f),
+                ("selection_bias", _vp)]
+
+
+class RopeRows(C.Structure):
+    """``berth_rope_rows`` of include/berth_b200.h."""
+    _fields_ = [("x", _vp), ("y", _vp), ("norm", _vp)] + [(n, _i64) for n in ("x_token", "x_head", "y_token", "y_head")] + [("heads", _i)]
+
+
+class RopeScaling(C.Structure):
+    """``berth_rope_scaling`` of include/berth_b200.h."""
+    _fields_ = [("kind", _i)] + [(n, C.c_double) for n in ("factor", "original_context", "beta_fast", "beta_slow", "low_factor",
+                                                            "high_factor", "attention_factor_override")]
+
+
 class TensorInfo(C.Structure):
     """``berth_tensor_info`` of include/berth_b200_checkpoint.h."""
     _fields_ = [("name", C.c_char_p), ("shard", C.c_char_p), ("dtype", _i), ("rank", _i), ("shape", _u64 * 8),
@@ -51,6 +68,7 @@ class ModelConfigStruct(C.Structure):
 
 
 _tip, _lip = C.POINTER(TensorInfo), C.POINTER(LinearInfo)
+_rrp, _mrp = C.POINTER(RopeRows), C.POINTER(MoeRouting)
 
 # name -> (restype, argtypes); every symbol the headers declare.
 SIGNATURES = {
@@ -85,6 +103,15 @@ SIGNATURES = {
     "berth_ops_rms_norm": (_i, [_vp] * 3 + [_i, _i, _f, _f, _f, _i, _vp]),
     "berth_ops_rms_norm_f16": (_i, [_vp] * 3 + [_i, _i, _f, _f, _f, _vp]),
     "berth_ops_rms_norm_res_in": (_i, [_vp] * 4 + [_i, _i, _f, _f, _f, _i, _vp]),
+    "berth_ops_rope": (_i, [_rrp, _rrp, _vp, _vp] + [_i] * 4 + [_f] * 3 + [_i, _vp]),
+    "berth_ops_rope_frequencies": (_i, [C.POINTER(C.c_double), _i, C.c_double, C.POINTER(RopeScaling), C.POINTER(C.c_float)]),
+    "berth_ops_logprobs": (_i, [_vp, _i, _i64, _vp, _f] + [_vp] * 5 + [_i] * 3 + [_vp]),
+    "berth_moe_route": (_i, [_vp, _i, _i64] + [_vp] * 3 + [_i] * 8 + [_f, _vp]),
+    "berth_moe_router_topk_routed": (_i, [_vp] * 3 + [_mrp] + [_vp] * 3 + [_i] * 4 + [_vp]),
+    "berth_moe_layer_routed": (_i, [C.POINTER(MoeWeights), _mrp, _vp, _i, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "berth_moe_ep_send_routed": (_i, [_vp, _i, _vp, _vp, _mrp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "berth_moe_p2p_send_routed": (_i, [_vp, _i, _vp, _vp, _mrp, _i, _i, _i, _vp, _vp, _vp, _i, _i, C.c_uint, _vp, _vp, _vp, _i, _vp, C.c_size_t,
+                                       _vp]),
     "berth_moe_router_topk": (_i, [_vp] * 6 + [_i] * 4 + [_vp]),
     "berth_moe_workspace_bytes": (C.c_size_t, [_i] * 6),
     "berth_moe_layer": (_i, [C.POINTER(MoeWeights), _vp, _i, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),

@@ -5,7 +5,7 @@
 // berth has the shape contract of this block but no operator; the arithmetic contract is the
 // one the CPU checker under oracle/ states (router summation order, tie rule, rounding points).
 #include "exl3_decode.cuh"
-#include "../../include/berth_b200.h"
+#include "route.cuh"
 
 #include <algorithm>
 
@@ -902,9 +902,9 @@ void check_moe_shapes(const berth_moe_weights* w, int T, bool routes = false)
     if (w->codebook < 0 || w->codebook > 2) throw std::runtime_error("moe: codebook must be 0, 1, or 2");
 }
 
-// Returns the names of the kernels that run.
-std::string router_topk(const void* x, const void* w_router, const float* bias, int32_t* topk_idx, float* topk_w, float* logits,
-                        int T, int H, int E, int k, cudaStream_t st)
+// Returns the names of the kernels that run.  routing (checked, may be null): how the experts are chosen from the logits.
+std::string router_topk(const void* x, const void* w_router, const float* bias, const berth_moe_routing* routing, int32_t* topk_idx,
+                        float* topk_w, float* logits, int T, int H, int E, int k, cudaStream_t st)
 {
     const size_t smem = size_t(kRouterTok) * H * 4 + size_t(32) * kRouterTok * 33 * 4;
     if (smem > 200 * 1024) throw std::runtime_error("moe router: hidden is too large for the router's shared-memory tile");
@@ -941,6 +941,7 @@ std::string router_topk(const void* x, const void* w_router, const float* bias, 
     else if (one_wave(8)) narrow(k_moe_router_logits<32, 8>, 32, 8);
     else narrow(k_moe_router_logits<16, 8>, 16, 8);
     cuda_ok(cudaGetLastError(), "k_moe_router_logits launch");
+    if (routing) return name + " + " + route_tokens(logits, true, E, *routing, topk_idx, topk_w, T, E, k, st);
     launch_pdl(E <= 128 ? k_moe_topk<4> : (E <= 256 ? k_moe_topk<8> : k_moe_topk<32>), dim3((T + 3) / 4), dim3(128), 0, st, "k_moe_topk launch", logits, topk_idx, topk_w, T, E, k);
     cuda_ok(cudaGetLastError(), "k_moe_topk launch");
     return name + " + k_moe_topk";
@@ -1105,6 +1106,13 @@ extern "C" const char* berth_moe_last_launch(void) { return moe_state().launch.c
 extern "C" int berth_moe_router_topk(const void* x, const void* w_router, const float* router_bias, int32_t* topk_idx,
                                      float* topk_w, float* logits, int T, int hidden, int n_experts, int top_k, void* stream)
 {
+    return berth_moe_router_topk_routed(x, w_router, router_bias, nullptr, topk_idx, topk_w, logits, T, hidden, n_experts, top_k, stream);
+}
+
+extern "C" int berth_moe_router_topk_routed(const void* x, const void* w_router, const float* router_bias, const berth_moe_routing* routing,
+                                            int32_t* topk_idx, float* topk_w, float* logits, int T, int hidden, int n_experts, int top_k,
+                                            void* stream)
+{
     CallState& st = moe_state();
     return guarded(st, [&] {
         if (!x || !w_router || !topk_idx || !topk_w || !logits) throw std::runtime_error("moe router: null device pointer");
@@ -1113,7 +1121,8 @@ extern "C" int berth_moe_router_topk(const void* x, const void* w_router, const 
         if (n_experts < 32 || n_experts % 32 || n_experts > 1024)
             throw std::runtime_error("moe router: n_experts must be a multiple of 32 up to 1024");
         if (top_k < 1 || top_k > 32 || top_k > n_experts) throw std::runtime_error("moe router: top_k must be in 1..=32");
-        st.launch = router_topk(x, w_router, router_bias, topk_idx, topk_w, logits, T, hidden, n_experts, top_k, (cudaStream_t) stream);
+        if (routing) check_routing(routing, n_experts, top_k);
+        st.launch = router_topk(x, w_router, router_bias, routing, topk_idx, topk_w, logits, T, hidden, n_experts, top_k, (cudaStream_t) stream);
     });
 }
 
@@ -1221,6 +1230,14 @@ extern "C" int berth_moe_ep_send(const void* x, int T, const void* w_router, con
                                  int top_k, int32_t* topk_idx, float* topk_w, int32_t* inv, void* send_rows, int32_t* counts,
                                  void* ws, size_t ws_bytes, void* stream)
 {
+    return berth_moe_ep_send_routed(x, T, w_router, router_bias, nullptr, hidden, n_experts, top_k, topk_idx, topk_w, inv, send_rows, counts, ws,
+                                    ws_bytes, stream);
+}
+
+extern "C" int berth_moe_ep_send_routed(const void* x, int T, const void* w_router, const float* router_bias, const berth_moe_routing* routing,
+                                        int hidden, int n_experts, int top_k, int32_t* topk_idx, float* topk_w, int32_t* inv, void* send_rows,
+                                        int32_t* counts, void* ws, size_t ws_bytes, void* stream)
+{
     CallState& st = moe_state();
     return guarded(st, [&] {
         if (!x || !w_router || !topk_idx || !topk_w || !inv || !send_rows || !counts || !ws)
@@ -1230,6 +1247,7 @@ extern "C" int berth_moe_ep_send(const void* x, int T, const void* w_router, con
         if (n_experts < 32 || n_experts % 32 || n_experts > 1024)
             throw std::runtime_error("moe ep send: n_experts must be a multiple of 32 up to 1024");
         if (top_k < 1 || top_k > 32 || top_k > n_experts) throw std::runtime_error("moe ep send: top_k must be in 1..=32");
+        if (routing) check_routing(routing, n_experts, top_k);
         if (ws_bytes < berth_moe_ep_send_workspace_bytes(T, n_experts, top_k)) throw std::runtime_error("moe ep send: workspace too small");
         cudaStream_t cs = (cudaStream_t) stream;
         const int R = T * top_k;
@@ -1243,11 +1261,11 @@ extern "C" int berth_moe_ep_send(const void* x, int T, const void* w_router, con
         es.n_problems = (int*) take(4);
         es.problems = (GemvProblem*) take((size_t(R) / 8 + n_experts + 1) * sizeof(GemvProblem));
         es.max_problems = R / 8 + n_experts;
-        router_topk(x, w_router, router_bias, topk_idx, topk_w, logits, T, hidden, n_experts, top_k, cs);
+        const std::string router = router_topk(x, w_router, router_bias, routing, topk_idx, topk_w, logits, T, hidden, n_experts, top_k, cs);
         dispatch(topk_idx, R, 0, n_experts, 8, es, perm, inv, cs);
         launch_pdl(k_moe_gather_rows, dim3(std::min(R, 148 * 8)), dim3(256), 0, cs, "k_moe_gather_rows launch", (const __half*) x, perm, es.offsets + n_experts, top_k, (__half*) send_rows, hidden);
         cuda_ok(cudaGetLastError(), "k_moe_gather_rows launch");
-        st.launch = "k_moe_router_logits + k_moe_topk + k_moe_count/scan/scatter + k_moe_gather_rows";
+        st.launch = (routing ? router : std::string("k_moe_router_logits + k_moe_topk")) + " + k_moe_count/scan/scatter + k_moe_gather_rows";
     });
 }
 
@@ -1379,6 +1397,15 @@ extern "C" int berth_moe_p2p_send(const void* x, int T, const void* w_router, co
                                   const void* const* cnt_all, const void* const* flags, const void* const* recv_rows, int max_rows,
                                   void* ws, size_t ws_bytes, void* stream)
 {
+    return berth_moe_p2p_send_routed(x, T, w_router, router_bias, nullptr, hidden, n_experts, top_k, topk_idx, topk_w, inv, rank, world, epoch, cnt_all,
+                                     flags, recv_rows, max_rows, ws, ws_bytes, stream);
+}
+
+extern "C" int berth_moe_p2p_send_routed(const void* x, int T, const void* w_router, const float* router_bias, const berth_moe_routing* routing,
+                                         int hidden, int n_experts, int top_k, int32_t* topk_idx, float* topk_w, int32_t* inv, int rank, int world,
+                                         unsigned epoch, const void* const* cnt_all, const void* const* flags, const void* const* recv_rows,
+                                         int max_rows, void* ws, size_t ws_bytes, void* stream)
+{
     CallState& st = moe_state();
     return guarded(st, [&] {
         if (!w_router || !ws || (T > 0 && (!x || !topk_idx || !topk_w || !inv))) throw std::runtime_error("moe p2p send: null device pointer");
@@ -1387,6 +1414,7 @@ extern "C" int berth_moe_p2p_send(const void* x, int T, const void* w_router, co
         if (top_k < 1 || top_k > 32 || top_k > n_experts) throw std::runtime_error("moe p2p send: top_k must be in 1..=32");
         const int n_local = world > 0 ? n_experts / world : 0;
         check_p2p_world(rank, world, n_experts, n_local);
+        if (routing) check_routing(routing, n_experts, top_k);
         if (ws_bytes < berth_moe_p2p_send_workspace_bytes(std::max(T, 1), n_experts, top_k, world))
             throw std::runtime_error("moe p2p send: workspace too small");
         const PeerPtrs pc = peer_ptrs(cnt_all, world, "count table"), pf = peer_ptrs(flags, world, "flag"), pr = peer_ptrs(recv_rows, world, "receive buffer");
@@ -1399,8 +1427,10 @@ extern "C" int berth_moe_p2p_send(const void* x, int T, const void* w_router, co
         ExpertScratch es{};
         es.counts = s.counts; es.offsets = s.offsets; es.n_problems = s.n_problems; es.problems = s.problems;
         es.max_problems = std::max(T, 1) * top_k / 8 + n_experts;   // as carve_p2p_send sized the table
+        std::string router = "k_moe_router_logits + k_moe_topk";
         if (T > 0) {
-            router_topk(x, w_router, router_bias, topk_idx, topk_w, s.logits, T, hidden, n_experts, top_k, cs);
+            const std::string ran = router_topk(x, w_router, router_bias, routing, topk_idx, topk_w, s.logits, T, hidden, n_experts, top_k, cs);
+            if (routing) router = ran;
             dispatch(topk_idx, R, 0, n_experts, 8, es, s.perm, inv, cs);
         } else {
             cuda_ok(cudaMemsetAsync(s.counts, 0, size_t(n_experts) * 4, cs), "moe p2p send: clear counts");
@@ -1414,7 +1444,7 @@ extern "C" int berth_moe_p2p_send(const void* x, int T, const void* w_router, co
         }
         k_ep_barrier<<<1, 32, 0, cs>>>(pf, 1, rank, world, epoch, status);
         cuda_ok(cudaGetLastError(), "k_ep_barrier launch");
-        st.launch = "k_moe_router_logits + k_moe_topk + k_moe_count/scan/scatter + k_ep_publish_tables + k_ep_dispatch + k_ep_barrier";
+        st.launch = router + " + k_moe_count/scan/scatter + k_ep_publish_tables + k_ep_dispatch + k_ep_barrier";
     });
 }
 
@@ -1510,9 +1540,16 @@ extern "C" size_t berth_moe_workspace_bytes(int T, int hidden, int inter, int sh
 extern "C" int berth_moe_layer(const berth_moe_weights* w, const void* x, int T, void* out, int32_t* topk_idx, float* topk_w,
                                void* workspace, size_t workspace_bytes, void* stream)
 {
+    return berth_moe_layer_routed(w, nullptr, x, T, out, topk_idx, topk_w, workspace, workspace_bytes, stream);
+}
+
+extern "C" int berth_moe_layer_routed(const berth_moe_weights* w, const berth_moe_routing* routing, const void* x, int T, void* out,
+                                      int32_t* topk_idx, float* topk_w, void* workspace, size_t workspace_bytes, void* stream)
+{
     CallState& st = moe_state();
     return guarded(st, [&] {
         check_moe_shapes(w, T, true);
+        if (routing) check_routing(routing, w->n_experts, w->top_k);
         if (!x || !out || !topk_idx || !topk_w || !workspace) throw std::runtime_error("moe layer: null device pointer");
         if (!w->w_router || !w->gate_trellis || !w->up_trellis || !w->down_trellis || !w->gate_suh || !w->gate_svh ||
             !w->up_suh || !w->up_svh || !w->down_suh || !w->down_svh)
@@ -1543,7 +1580,7 @@ extern "C" int berth_moe_layer(const berth_moe_weights* w, const void* x, int T,
         ExpertScratch es = carve_experts(b, RT, NM, H, I, plan);
         b += carve_experts(nullptr, R + T, E + 1, H, I, plan).bytes;
 
-        const std::string router = router_topk(x, w->w_router, w->router_bias, topk_idx, topk_w, logits, T, H, E, K, cs);
+        const std::string router = router_topk(x, w->w_router, w->router_bias, routing, topk_idx, topk_w, logits, T, H, E, K, cs);
         const bool paired = up_behind_gate(w, NM);
         dispatch(topk_idx, R, 0, E, plan.chunk, es, perm, inv, cs, fused_shared ? T : 0, paired ? RT : 0, NM);
         // the rotation kernel of gate and up gathers the routed rows (and the shared expert's) from x itself

@@ -51,6 +51,33 @@ def _s(b) -> str:
     return (b or b"").decode("utf-8", "replace")
 
 
+def _device_of(what: str, *tensors) -> None:
+    """The callers that take shapes and strides from torch tensors: all of them on the current CUDA device, which is the one
+    the library launches on."""
+    import torch
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise Error(f"{what}: every tensor must be on the CUDA device")
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise Error(f"{what}: a tensor is on device {t.get_device()}, the current device is {device}")
+
+
+def _flat(what: str, name: str, t, dtype, *shape) -> None:
+    if t is not None and (t.dtype is not dtype or tuple(t.shape) != shape or not t.is_contiguous()):
+        raise Error(f"{what}: {name} must be a contiguous {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _is_f32(what: str, t) -> int:
+    import torch
+    if t.dtype is torch.float32:
+        return 1
+    if t.dtype is torch.float16:
+        return 0
+    raise Error(f"{what}: fp16 or fp32 is expected, got {t.dtype}")
+
+
 def last_launch() -> str:
     return _s(_lib.lib().berth_exl3_last_launch())
 
@@ -328,3 +355,89 @@ class ops:
                                                   constant_scale, 1 if weight_bf16 else 0, _stream(stream))
         if rc != 0:
             raise Error(ops.last_error() or f"rms_norm_res_in launch failed ({rc})")
+
+    @staticmethod
+    def rope(q, k, positions, inv_freq, q_out, k_out, interleaved: bool = False, attention_factor: float = 1.0, q_norm=None, k_norm=None,
+             norm_epsilon: float = 1e-6, norm_bias: float = 0.0, stream=None) -> None:
+        """Rotary positions of ``q`` and ``k`` (``k`` may be ``None``), with the RMSNorm of every head before them where ``q_norm`` /
+        ``k_norm`` (bfloat16 ``[head_dim]``) is given.  Tensors ``[tokens][heads][head_dim]`` of any strides with contiguous heads,
+        fp16 or fp32; the outputs may be the inputs themselves.  ``positions`` int32 ``[tokens]``; ``inv_freq`` float64, one entry per
+        pair (``rope_frequencies``), so ``2 * len(inv_freq)`` elements of a head turn: neighbours when ``interleaved``, else i and
+        i + len(inv_freq).  The formulas are at ``berth_ops_rope`` in include/berth_b200.h."""
+        import torch
+        _device_of("rope", q, k, positions, inv_freq, q_out, k_out, q_norm, k_norm)
+        if q.dim() != 3:
+            raise Error(f"rope: q must be [tokens][heads][head_dim], got {tuple(q.shape)}")
+        tokens, dim, f32 = q.shape[0], q.shape[2], _is_f32("rope", q)
+        if positions.dtype is not torch.int32 or positions.dim() != 1 or positions.shape[0] != tokens or not positions.is_contiguous():
+            raise Error("rope: positions must be a contiguous int32 tensor with one entry per token")
+        if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+            raise Error("rope: inv_freq must be a contiguous float64 tensor of one dimension")
+        if (k is None) != (k_out is None) or (k is None and k_norm is not None):
+            raise Error("rope: k, k_out and k_norm go together")
+        rows = []
+        for x, y, norm in ((q, q_out, q_norm), (k, k_out, k_norm)):
+            if x is None:
+                continue
+            if x.dtype is not q.dtype or y.dtype is not q.dtype or x.shape != y.shape or x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != dim:
+                raise Error("rope: q, k and their outputs must share type, tokens and head_dim, and an output its input's shape")
+            if dim > 1 and (x.stride(2) != 1 or y.stride(2) != 1):
+                raise Error("rope: the elements of a head must be contiguous")
+            if norm is not None:
+                _flat("rope", "a norm", norm, torch.bfloat16, dim)
+            xs, ys = x.stride(), y.stride()
+            rows.append(_lib.RopeRows(x.data_ptr(), y.data_ptr(), None if norm is None else norm.data_ptr(), xs[0], xs[1], ys[0], ys[1], x.shape[1]))
+        rc = _lib.lib().berth_ops_rope(rows[0], rows[1] if len(rows) > 1 else None, positions.data_ptr(), inv_freq.data_ptr(), tokens, dim,
+                                       2 * inv_freq.shape[0], interleaved, attention_factor, norm_epsilon, norm_bias, f32, _stream(stream))
+        if rc != 0:
+            raise Error(ops.last_error() or f"rope launch failed ({rc})")
+
+    ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
+
+    @staticmethod
+    def rope_frequencies(rot_dim: int, base: float, scaling: str = "none", factor: float = 1.0, original_context: float = 0.0,
+                         beta_fast: float = 32.0, beta_slow: float = 1.0, low_factor: float = 1.0, high_factor: float = 4.0,
+                         attention_factor: float = 0.0) -> tuple:
+        """``(inv_freq, attention_factor)`` for :meth:`rope`: a list of ``rot_dim / 2`` floats to put on the device once as float64, and
+        the factor on cos and sin.  No CUDA call; the kinds of scaling are at ``berth_ops_rope_frequencies``."""
+        import ctypes as C
+        if scaling not in ops.ROPE_SCALING:
+            raise Error(f"rope frequencies: scaling must be one of {', '.join(ops.ROPE_SCALING)}, got {scaling!r}")
+        out, af = (C.c_double * max(1, rot_dim // 2))(), C.c_float()
+        sc = _lib.RopeScaling(ops.ROPE_SCALING[scaling], factor, original_context, beta_fast, beta_slow, low_factor, high_factor, attention_factor)
+        if _lib.lib().berth_ops_rope_frequencies(out, rot_dim, base, C.byref(sc), C.byref(af)) != 0:
+            raise Error(ops.last_error())
+        return list(out), af.value
+
+    @staticmethod
+    def logprobs(logits, tokens, logprob, rank, entropy, top_idx, top_logprob, vocab: int | None = None, inv_temp: float = 1.0, stream=None) -> None:
+        """Log probabilities under ``softmax(logits * inv_temp)`` in one pass over ``logits`` (fp16 or fp32 ``[rows][>= vocab]``, rows of any
+        stride; ``vocab`` defaults to all columns): ``logprob`` fp32 and ``rank`` int32 ``[rows]`` of ``tokens`` (int32 ``[rows]``),
+        ``entropy`` fp32 ``[rows]``, ``top_idx`` int32 and ``top_logprob`` fp32 ``[rows][n]``, n <= 32, the best alternatives.  Any output
+        may be ``None``.  Masks, ties and padding tokens: ``berth_ops_logprobs`` in include/berth_b200.h."""
+        import torch
+        _device_of("logprobs", logits, tokens, logprob, rank, entropy, top_idx, top_logprob)
+        if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise Error("logprobs: logits must be [rows][vocab] with contiguous rows")
+        rows, cols = logits.shape
+        vocab = cols if vocab is None else vocab
+        if vocab > cols:
+            raise Error(f"logprobs: vocab {vocab} exceeds the {cols} columns of logits")
+        f32 = _is_f32("logprobs", logits)
+        _flat("logprobs", "tokens", tokens, torch.int32, rows)
+        _flat("logprobs", "logprob", logprob, torch.float32, rows)
+        _flat("logprobs", "rank", rank, torch.int32, rows)
+        _flat("logprobs", "entropy", entropy, torch.float32, rows)
+        if (top_idx is None) != (top_logprob is None):
+            raise Error("logprobs: top_idx and top_logprob go together")
+        n = 0
+        if top_idx is not None:
+            if top_idx.dim() != 2:
+                raise Error("logprobs: top_idx must be [rows][n]")
+            n = top_idx.shape[1]
+            _flat("logprobs", "top_idx", top_idx, torch.int32, rows, n)
+            _flat("logprobs", "top_logprob", top_logprob, torch.float32, rows, n)
+        rc = _lib.lib().berth_ops_logprobs(logits.data_ptr(), f32, logits.stride(0), _ptr(tokens), inv_temp, _ptr(logprob), _ptr(rank), _ptr(entropy),
+                                           _ptr(top_idx) if n else None, _ptr(top_logprob) if n else None, n, rows, vocab, _stream(stream))
+        if rc != 0:
+            raise Error(ops.last_error() or f"logprobs launch failed ({rc})")

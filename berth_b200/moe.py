@@ -14,7 +14,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .kernels import Error, _s
+from .kernels import Error, _device_of, _flat, _is_f32, _ptr, _s, _stream
 
 _PTR_FIELDS = [n for n, _ in _lib.MoeWeights._fields_[7:]]
 
@@ -40,11 +40,64 @@ def router_topk(x, w_router, router_bias, topk_idx, topk_w, logits, T, hidden, n
         raise Error(last_error() or f"moe router launch failed ({rc})")
 
 
+SCORES = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORES = {"max": 0, "top2": 1}
+
+
+def _choice(score: str, group_score: str) -> tuple:
+    if score not in SCORES:
+        raise Error(f"moe route: score must be one of {', '.join(SCORES)}, got {score!r}")
+    if group_score not in GROUP_SCORES:
+        raise Error(f"moe route: group_score must be one of {', '.join(GROUP_SCORES)}, got {group_score!r}")
+    return SCORES[score], GROUP_SCORES[group_score]
+
+
+def route(logits, selection_bias, topk_idx, topk_w, top_k: int, score: str = "softmax", n_group: int = 1, topk_group: int = 1,
+          group_score: str = "max", renormalize: bool = True, scale: float = 1.0, stream=None) -> None:
+    """The experts of every token from its router logits (fp16 or fp32 ``[T][n_experts]``, rows of any stride): ``topk_idx`` int32 and
+    ``topk_w`` fp32 ``[T][top_k]``.  ``selection_bias`` (fp32 ``[n_experts]`` or ``None``) takes part in the choice only.  The formulas
+    and what happens to masked and NaN logits are at ``berth_moe_routing`` in include/berth_b200.h."""
+    _device_of("moe route", logits, selection_bias, topk_idx, topk_w)
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise Error("moe route: logits must be [T][n_experts] with contiguous rows")
+    T, E = logits.shape
+    f32 = _is_f32("moe route", logits)
+    _flat("moe route", "selection_bias", selection_bias, torch.float32, E)
+    _flat("moe route", "topk_idx", topk_idx, torch.int32, T, top_k)
+    _flat("moe route", "topk_w", topk_w, torch.float32, T, top_k)
+    sc, gs = _choice(score, group_score)
+    rc = _lib.lib().berth_moe_route(logits.data_ptr(), f32, logits.stride(0), _ptr(selection_bias), topk_idx.data_ptr(), topk_w.data_ptr(), T, E,
+                                    top_k, sc, n_group, topk_group, gs, renormalize, scale, _stream(stream))
+    if rc != 0:
+        raise Error(last_error() or f"moe route launch failed ({rc})")
+
+
+class Routing:
+    """How a layer chooses its experts where that is not the softmax over the k largest logits: :func:`route`'s choice, for
+    ``MoeLayer`` and ``GpuStages``.  ``selection_bias`` covers all the layer's experts (a tensor, or an array to upload)."""
+
+    def __init__(self, score: str = "softmax", n_group: int = 1, topk_group: int = 1, group_score: str = "max", renormalize: bool = True,
+                 scale: float = 1.0, selection_bias=None):
+        sc, gs = _choice(score, group_score)
+        self.fields = (sc, n_group, topk_group, gs, int(renormalize), scale)
+        self.selection_bias = selection_bias
+
+    def on(self, device: torch.device, n_experts: int) -> tuple:
+        """(``berth_moe_routing`` for ``device``, the bias tensor that it points to)."""
+        b = self.selection_bias
+        if b is not None:
+            b = torch.as_tensor(b).to(device=device, dtype=torch.float32).contiguous()
+            if tuple(b.shape) != (n_experts,):
+                raise Error(f"moe route: selection_bias must have {n_experts} entries, got {tuple(b.shape)}")
+        return _lib.MoeRouting(*self.fields, None if b is None else b.data_ptr()), b
+
+
 class MoeLayer:
     """One MoE layer resident on a GPU.  ``weights`` is the dict of ``berth_b200.synth.moe_layer_weights``
     (or the same keys filled from a checkpoint): numpy arrays are uploaded, torch tensors are kept."""
 
-    def __init__(self, device: torch.device, weights: dict, max_tokens: int, fuse_shared: bool = True, pair_gate_up: bool = True):
+    def __init__(self, device: torch.device, weights: dict, max_tokens: int, fuse_shared: bool = True, pair_gate_up: bool = True,
+                 routing: Routing | None = None):
         self.device = device
         self.dims = {k: int(weights[k]) for k in ("hidden", "inter", "shared_inter", "n_experts", "top_k", "bits", "cb")}
         self._keep = {}
@@ -99,6 +152,7 @@ class MoeLayer:
                     if f"sh_{p}_{k}" in stacked:
                         self._keep[f"sh_{p}_{k}"] = part[n - 1]
                         setattr(self.c, f"sh_{p}_{k}", part[n - 1].data_ptr())
+        self.routing, self._selection_bias = (None, None) if routing is None else routing.on(device, self.dims["n_experts"])
         self.max_tokens = 0
         self._alloc(max_tokens)
 
@@ -116,9 +170,9 @@ class MoeLayer:
         T = x.shape[0]
         if T > self.max_tokens:
             self._alloc(T)
-        rc = _lib.lib().berth_moe_layer(C.byref(self.c), x.data_ptr(), T, out.data_ptr(), topk_idx.data_ptr(),
-                                        topk_w.data_ptr(), self.workspace.data_ptr(), self.workspace.numel(),
-                                        None if stream is None else stream.cuda_stream)
+        rc = _lib.lib().berth_moe_layer_routed(C.byref(self.c), self.routing, x.data_ptr(), T, out.data_ptr(), topk_idx.data_ptr(),
+                                               topk_w.data_ptr(), self.workspace.data_ptr(), self.workspace.numel(),
+                                               None if stream is None else stream.cuda_stream)
         if rc != 0:
             raise Error(last_error() or f"moe layer launch failed ({rc})")
 
@@ -143,8 +197,10 @@ class GpuStages:
     rank's expert stacks (``n_experts`` = number of LOCAL experts), the full router and the shared
     expert."""
 
-    def __init__(self, device: torch.device, weights: dict, n_experts_total: int, max_rows: int, max_rows_per_expert: int):
+    def __init__(self, device: torch.device, weights: dict, n_experts_total: int, max_rows: int, max_rows_per_expert: int,
+                 routing: Routing | None = None):
         self.device = device
+        self.routing, self._selection_bias = (None, None) if routing is None else routing.on(device, n_experts_total)
         self.layer = MoeLayer.__new__(MoeLayer)
         MoeLayer.__init__(self.layer, device, weights, 1)
         self.d = self.layer.dims
@@ -178,7 +234,10 @@ class GpuStages:
         idx = torch.empty((T, k), dtype=torch.int32, device=self.device)
         w = torch.empty((T, k), dtype=torch.float32, device=self.device)
         logits = torch.empty((T, self.E), dtype=torch.float32, device=self.device)
-        router_topk(x, self.layer._keep["w_router"], self.layer._keep.get("router_bias"), idx, w, logits, T, H, self.E, k)
+        kp = self.layer._keep
+        bias = kp.get("router_bias")
+        self._check(_lib.lib().berth_moe_router_topk_routed(x.data_ptr(), kp["w_router"].data_ptr(), _ptr(bias), self.routing, idx.data_ptr(),
+                                                            w.data_ptr(), logits.data_ptr(), T, H, self.E, k, _cur_stream(self.device)))
         return idx, w
 
     def rows_hint(self, n_rows: int, n_local: int) -> int:
@@ -266,9 +325,9 @@ class GpuStages:
         counts = torch.empty(E, dtype=torch.int32, device=self.device)
         kp = self.layer._keep
         bias = kp.get("router_bias")
-        self._check(l.berth_moe_ep_send(x.data_ptr(), T, kp["w_router"].data_ptr(), None if bias is None else bias.data_ptr(), H, E, k,
-                                        idx.data_ptr(), w.data_ptr(), inv.data_ptr(), rows.data_ptr(), counts.data_ptr(),
-                                        self._send_ws.data_ptr(), self._send_ws.numel(), _cur_stream(self.device)))
+        self._check(l.berth_moe_ep_send_routed(x.data_ptr(), T, kp["w_router"].data_ptr(), _ptr(bias), self.routing, H, E, k, idx.data_ptr(),
+                                               w.data_ptr(), inv.data_ptr(), rows.data_ptr(), counts.data_ptr(), self._send_ws.data_ptr(),
+                                               self._send_ws.numel(), _cur_stream(self.device)))
         return idx, w, inv, rows, counts
 
     def shared_is_stacked(self) -> bool:
@@ -484,9 +543,9 @@ class P2pMoeLayer:
         kp = st.layer._keep
         bias = kp.get("router_bias")
         p = lambda t: t.data_ptr() if t.numel() else None
-        st._check(l.berth_moe_p2p_send(p(x), T, kp["w_router"].data_ptr(), None if bias is None else bias.data_ptr(), H, self.E, k,
-                                       p(idx), p(w), inv.data_ptr(), self.rank, self.world, self.epoch, self.cnt_ptrs, self.flag_ptrs,
-                                       self.recv_ptrs, self.max_rows, self.send_ws.data_ptr(), self.send_ws.numel(), _cur_stream(dev)))
+        st._check(l.berth_moe_p2p_send_routed(p(x), T, kp["w_router"].data_ptr(), _ptr(bias), st.routing, H, self.E, k, p(idx), p(w), inv.data_ptr(),
+                                              self.rank, self.world, self.epoch, self.cnt_ptrs, self.flag_ptrs, self.recv_ptrs, self.max_rows,
+                                              self.send_ws.data_ptr(), self.send_ws.numel(), _cur_stream(dev)))
         if self.profile:
             self._ev[1].record()
         stacked = st.shared_is_stacked() and T > 0

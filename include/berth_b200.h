@@ -247,6 +247,63 @@ int berth_ops_rms_norm_f16(const void* x, const void* weight, void* y, int rows,
 int berth_ops_rms_norm_res_in(const void* x, const void* weight, void* y, void* residual, int rows, int dim,
                               float epsilon, float constant_bias, float constant_scale, int weight_bf16,
                               void* stream);
+/* Rotary positions of the q and k rows of an attention block, optionally with their per-head RMSNorm, in one launch
+ * (no counterpart in this library's part of berth; berth's attention glue is crates/berth-kernels/csrc/attn/rope.cu).
+ * For every token t and head h, with x the head's head_dim values (after the norm, unrounded) and pair i < rot_dim / 2:
+ *   angle = positions[t] * inv_freq[i]                                   (64 bits, reduced to one turn before cos and sin)
+ *   y_a = attention_factor * (x_a * cos - x_b * sin),  y_b = attention_factor * (x_b * cos + x_a * sin)
+ * with (a, b) = (i, i + rot_dim / 2), or (2i, 2i + 1) when interleaved != 0; the elements from rot_dim on are passed on.
+ * Norm (norm != NULL, bfloat16 [head_dim]): x = x * r * (norm + norm_bias), r = 1 / sqrt(mean(x^2) + norm_epsilon),
+ * as berth_ops_rms_norm_f16 over rows of one head, but not rounded to fp16 before the rotation.
+ * One berth_rope_rows describes q or k: x and y of the same type (fp16, or fp32 when fp32 != 0), element strides between
+ * tokens and heads for each, so that rows may be columns of a wider buffer or slots of a cache; the head_dim elements
+ * of a head are contiguous.  y may be x itself (with x's strides); any other overlap of outputs with inputs, or of two
+ * heads of an output, is undefined.  k may be NULL.  norm of q and of k are independent of each other.
+ * positions int32 [n_tokens], any value; inv_freq fp64 [rot_dim / 2]; both device memory.  head_dim up to 512, rot_dim
+ * even and at most head_dim.  Rows whose pointers and strides are multiples of 16 bytes take the wide accesses.
+ * Touches nothing but the tensors; launches on different streams are independent. */
+typedef struct berth_rope_rows {
+    const void* x;
+    void* y;
+    const void* norm;
+    int64_t x_token, x_head, y_token, y_head;
+    int heads;
+} berth_rope_rows;
+int berth_ops_rope(const berth_rope_rows* q, const berth_rope_rows* k, const int32_t* positions, const double* inv_freq,
+                   int n_tokens, int head_dim, int rot_dim, int interleaved, float attention_factor, float norm_epsilon,
+                   float norm_bias, int fp32, void* stream);
+/* The frequencies of berth_ops_rope on the HOST (no CUDA call): inv_freq[i] = base^(-2i / rot_dim), scaled for contexts
+ * longer than the trained one.  scaling NULL or kind 0: unscaled.  kind 1: every frequency divided by factor.  kind 2:
+ * base * factor^(rot_dim / (rot_dim - 2)) in the place of base (rot_dim > 2).  kind 3: frequencies that turn at least
+ * beta_fast times within original_context are kept, those of at most beta_slow turns divided by factor, a linear blend
+ * over the pair index between the two (bounds rounded outwards to whole pairs), and *attention_factor =
+ * 0.1 ln(factor) + 1 unless attention_factor_override > 0.  kind 4: kept above high_factor turns, divided by factor below low_factor turns,
+ * in between blended by (turns - low_factor) / (high_factor - low_factor).  *attention_factor (may be NULL) is 1 for the
+ * other kinds.  -1 and berth_ops_last_error for values out of range. */
+typedef struct berth_rope_scaling {
+    int kind;
+    double factor, original_context, beta_fast, beta_slow, low_factor, high_factor, attention_factor_override;
+} berth_rope_scaling;
+int berth_ops_rope_frequencies(double* inv_freq, int rot_dim, double base, const berth_rope_scaling* scaling,
+                               float* attention_factor);
+/* Log probabilities of the distribution softmax(logits * inv_temp) of every row, in one pass over the logits: what an
+ * lm_head's rows say about given tokens (no counterpart in berth; its sampler only draws a token).
+ *   tokens       int32 [rows] or NULL: logprob[r] = ln p(tokens[r]); rank[r] = how many tokens come before it in the
+ *                row's order (larger logit first, then the lower token), so 0 is the arg-max.  A token outside
+ *                [0, vocab) (the padding of a batch): logprob 0, rank -1.
+ *   entropy      fp32 [rows] or NULL: -sum p ln p in nats.
+ *   top_idx, top_logprob   int32 / fp32 [rows][top_n]: the first top_n tokens of that order and their ln p
+ *                (top_n <= 32 and at most vocab; 0: both unused).
+ * logits fp16, or fp32 when logits_fp32 != 0; row r starts at element r * row_stride; elements from vocab on are not
+ * read.  logprob and rank may be NULL.  inv_temp positive and at most 1e30.
+ * -inf logits are masked tokens: ln p = -inf, nothing added to the entropy.  A row that is masked altogether gives
+ * ln p = -inf throughout, entropy 0, and the lowest tokens as alternatives.  A row with a NaN or +inf logit gives NaN for
+ * every real number; its whole numbers stay in range (NaN after everything else in the order; rank -1 for a NaN token).
+ * Needs no workspace: a row is split over the blocks of a cluster, which join in shared memory; two launches or
+ * captured graphs share nothing.  The order of every sum is fixed: the same call repeats its bits. */
+int berth_ops_logprobs(const void* logits, int logits_fp32, int64_t row_stride, const int32_t* tokens, float inv_temp,
+                       float* logprob, int32_t* rank, float* entropy, int32_t* top_idx, float* top_logprob, int top_n,
+                       int rows, int vocab, void* stream);
 const char* berth_ops_last_error(void);
 const char* berth_ops_last_launch(void);
 
@@ -311,6 +368,37 @@ typedef struct berth_moe_weights {
 int berth_moe_router_topk(const void* x, const void* w_router, const float* router_bias,
                           int32_t* topk_idx, float* topk_w, float* logits, int T, int hidden,
                           int n_experts, int top_k, void* stream);
+/* How the k experts of a token are chosen and weighted from its logits, where that is not the softmax over the k largest
+ * logits of berth_moe_router_topk.  With score s = softmax or sigmoid of the logits and choice c = s + selection_bias:
+ * the experts stand in n_group groups of consecutive experts, a group is worth its best c (group_score 0) or the sum of
+ * its two best (1), and the topk_group best groups are kept; the top_k experts of largest c in them are chosen, and a
+ * chosen expert's weight is scale * s, or with renormalize scale * s / (sum of s over the chosen).  The bias takes part
+ * in the choice only.  Ties go to the lower group and the lower expert.
+ * Without bias, and unless groups are dropped by the sum of their two best, the order is that of the logits themselves;
+ * else choice scores are told apart as evaluated in double precision, whatever the type of the logits.
+ * Logits: +inf counts as the largest finite value.  -inf masks an expert: it is chosen only where nothing else is left,
+ * and its weight is 0; one masked altogether gives the lowest experts with weights 0.  A masked expert adds nothing to
+ * a group's sum.  A NaN logit comes last in the order and makes every weight of its row NaN.  The k indices of a row
+ * are always distinct and inside [0, n_experts). */
+typedef struct berth_moe_routing {
+    int score;                    /* 0 = softmax, 1 = sigmoid */
+    int n_group, topk_group;      /* 1, 1: no groups; n_group <= 32 divides n_experts, top_k <= topk_group * n_experts / n_group */
+    int group_score;              /* 0 = best, 1 = sum of the two best (groups of at least two experts) */
+    int renormalize;
+    float scale;
+    const float* selection_bias;  /* fp32 [n_experts], device, or NULL */
+} berth_moe_routing;
+/* The choice alone, from given logits: fp16, or fp32 when logits_fp32 != 0, row t at element t * row_stride; any
+ * n_experts up to 1024, top_k up to 32.  topk_idx int32 [T][k] in the order of the choice, topk_w fp32 [T][k].  Needs no
+ * workspace. */
+int berth_moe_route(const void* logits, int logits_fp32, int64_t row_stride, const float* selection_bias,
+                    int32_t* topk_idx, float* topk_w, int T, int n_experts, int top_k, int score, int n_group,
+                    int topk_group, int group_score, int renormalize, float scale, void* stream);
+/* berth_moe_router_topk, berth_moe_layer, berth_moe_ep_send and berth_moe_p2p_send with that choice in the place of
+ * theirs; routing NULL: exactly theirs.  selection_bias and n_group are those of all the layer's experts. */
+int berth_moe_router_topk_routed(const void* x, const void* w_router, const float* router_bias,
+                                 const berth_moe_routing* routing, int32_t* topk_idx, float* topk_w, float* logits, int T,
+                                 int hidden, int n_experts, int top_k, void* stream);
 /* Bytes of caller-provided scratch berth_moe_layer needs for T tokens (the library allocates
  * nothing per layer). */
 size_t berth_moe_workspace_bytes(int T, int hidden, int inter, int shared_inter, int n_experts,
@@ -321,6 +409,8 @@ size_t berth_moe_workspace_bytes(int T, int hidden, int inter, int shared_inter,
  * order, shared expert last. */
 int berth_moe_layer(const berth_moe_weights* w, const void* x, int T, void* out, int32_t* topk_idx,
                     float* topk_w, void* workspace, size_t workspace_bytes, void* stream);
+int berth_moe_layer_routed(const berth_moe_weights* w, const berth_moe_routing* routing, const void* x, int T, void* out,
+                           int32_t* topk_idx, float* topk_w, void* workspace, size_t workspace_bytes, void* stream);
 /* The stages of the layer one by one, for hosts that put a collective between them (expert
  * parallelism).  `ews` is caller-provided scratch of berth_moe_experts_workspace_bytes(max_rows,
  * n_local, hidden, inter, max_rows_per_expert) bytes; the same five values must be passed to
@@ -360,6 +450,10 @@ size_t berth_moe_ep_send_workspace_bytes(int T, int n_experts, int top_k);
 int berth_moe_ep_send(const void* x, int T, const void* w_router, const float* router_bias, int hidden,
                       int n_experts, int top_k, int32_t* topk_idx, float* topk_w, int32_t* inv,
                       void* send_rows, int32_t* counts, void* ws, size_t ws_bytes, void* stream);
+int berth_moe_ep_send_routed(const void* x, int T, const void* w_router, const float* router_bias,
+                             const berth_moe_routing* routing, int hidden, int n_experts, int top_k, int32_t* topk_idx,
+                             float* topk_w, int32_t* inv, void* send_rows, int32_t* counts, void* ws, size_t ws_bytes,
+                             void* stream);
 size_t berth_moe_ep_experts_workspace_bytes(int max_rows, int max_tokens, int world, int n_local,
                                             int hidden, int inter);
 int berth_moe_ep_experts(const berth_moe_weights* w, const void* recv_rows, int n_rows,
@@ -386,6 +480,11 @@ int berth_moe_p2p_send(const void* x, int T, const void* w_router, const float* 
                        int n_experts, int top_k, int32_t* topk_idx, float* topk_w, int32_t* inv, int rank,
                        int world, unsigned epoch, const void* const* cnt_all, const void* const* flags,
                        const void* const* recv_rows, int max_rows, void* ws, size_t ws_bytes, void* stream);
+int berth_moe_p2p_send_routed(const void* x, int T, const void* w_router, const float* router_bias,
+                              const berth_moe_routing* routing, int hidden, int n_experts, int top_k, int32_t* topk_idx,
+                              float* topk_w, int32_t* inv, int rank, int world, unsigned epoch,
+                              const void* const* cnt_all, const void* const* flags, const void* const* recv_rows,
+                              int max_rows, void* ws, size_t ws_bytes, void* stream);
 size_t berth_moe_p2p_experts_workspace_bytes(int max_rows, int n_local, int hidden, int inter);
 int berth_moe_p2p_experts(const berth_moe_weights* w, const void* x_local, int T_local, void* ysh, int rank,
                           int world, unsigned epoch, int n_experts_total, int top_k, int send_tokens,
