@@ -2,12 +2,12 @@
 //
 // A row is split over the CTAs of a cluster.  Every thread walks its 16-byte vectors with a running maximum M and the sums
 // z = sum 2^y and t = sum 2^y y, y = (x - M) * inv_temp * log2 e: ln p = (x - m) * inv_temp - ln z and the entropy
-// ln z - t / z * ln 2 follow from the joined (m, z, t).  Both sums grow in 64 bits from sums of 32 elements that are added
-// as a tree in 32: a certain row has z = 1 + little, and its entropy is made of that little.  The rank of a given token is a
-// count of the logits before it, taken in the same walk.
+// ln z - t / z * ln 2 follow from the joined (m, z, t).  A thread adds its vectors' sums, trees of 16 or 32, with the rounding
+// kept aside, and joins carry z less the maximum's own 1: a certain row has z = 1 + little, and its entropy is made of that
+// little.  The rank of a given token is a count of the logits before it, taken in the same walk.
 //
-// The n best come out of the walk's by-product, the threads' maxima.  The cluster's warps fall into at least n groups; the
-// smallest of the groups' maxima is a value that n logits reach, and few more do, all of them in threads whose maximum
+// The n best come out of the walk's by-product, the threads' maxima.  The cluster's warps fall into at least n groups (or
+// give their k largest threads each, where there are fewer warps than n); the smallest of the groups' maxima is a value that n logits reach, and few more do, all of them in threads whose maximum
 // reaches it.  Only those threads' vectors are read again (from L2, a few percent of the row), what reaches the value goes to
 // the first CTA's shared memory, and each finds its place by counting the larger ones.  Rows where too many reach it (equal
 // logits, a mask that leaves fewer than n) are scanned once more with a sorted list of 32 per warp instead.
@@ -21,7 +21,7 @@ namespace berth {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
-constexpr int kMaxTop = 32, kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 16, kKeys = 512;
+constexpr int kMaxTop = 32, kMaxCluster = 16, kKeys = 512;
 static_assert(kMaxCluster * kMaxTop <= kKeys, "the lists of a cluster share the key buffer");
 
 struct LogprobParams {
@@ -88,35 +88,42 @@ __device__ __forceinline__ unsigned peer_add(uint32_t a, unsigned v)
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// Running maximum and sums of a part of a row.
+// A part of a row: its maximum m, z = sum 2^y less the 1 of the maximum itself, t = sum 2^y y, y relative to m.  Without the 1,
+// fp32 keeps the small rest of a certain row to its own 2^-24.  m = -inf: no logit above it, z = 0 (NaN after a NaN).
 struct Part {
-    float m;       // -inf: no logit above it yet
-    double z, t;
+    float m, z, t;
 };
-// p brought to the maximum m >= p.m.  A part without a maximum has z = 0 (or NaN, which stays).
-__device__ __forceinline__ Part brought_to(Part p, float m, float scale2)
+__device__ __forceinline__ float redux_max(float v) { float r; asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float redux_min(float v) { float r; asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+// p, whose maximum is not the one that keeps its 1 out of the sum, relative to the maximum m.
+__device__ __forceinline__ Part beside(Part p, float m, float scale2)
 {
     if (p.m > -INFINITY) {
-        const float d = (p.m - m) * scale2;
-        const double f = ex2(d);
-        p.t = f > 0.0 ? (p.t + double(d) * p.z) * f : p.z * f;   // (a factor that vanished leaves 0, or NaN)
-        p.z *= f;
+        const float d = (p.m - m) * scale2, f = ex2(d), all = 1.f + p.z;
+        p.t = f != 0.f ? (p.t + d * all) * f : all * f;   // a factor that vanished leaves 0, or NaN
+        p.z = all * f;
     }
-    p.m = m;
     return p;
 }
-template <int LANES>
-__device__ __forceinline__ Part joined(Part p, float scale2)   // over groups of LANES lanes
+__device__ __forceinline__ Part joined(const Part& a, const Part& b, float scale2)
 {
-    float m = p.m;
+    const bool first = a.m >= b.m;
+    const Part &h = first ? a : b, o = beside(first ? b : a, h.m, scale2);
+    return Part{h.m, h.z + o.z, h.t + o.t};
+}
+// The parts of the warp's lanes as one, in every lane (the order of the sums is fixed).
+__device__ __forceinline__ Part joined(Part p, float scale2)
+{
+    const float m = redux_max(p.m);
+    const int holder = __ffs(__ballot_sync(dq::kFull, p.m == m)) - 1;
+    if (int(threadIdx.x & 31) != holder) p = beside(p, m, scale2);
 #pragma unroll
-    for (int off = LANES / 2; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(dq::kFull, m, off));
-    p = brought_to(p, m, scale2);
-#pragma unroll
-    for (int off = LANES / 2; off >= 1; off >>= 1) {
+    for (int off = 16; off >= 1; off >>= 1) {
         p.z += __shfl_xor_sync(dq::kFull, p.z, off);
         p.t += __shfl_xor_sync(dq::kFull, p.t, off);
     }
+    p.m = m;
     return p;
 }
 
@@ -130,6 +137,7 @@ template <> struct Vec<true> {
         const uint4 v = __ldcg(a);
         x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
     }
+    __device__ __forceinline__ void clear() { x[0] = x[1] = x[2] = x[3] = -INFINITY; }
     __device__ __forceinline__ f2 pair(int i) const { return pack2(x[2 * i], x[2 * i + 1]); }
     __device__ __forceinline__ float at(int i) const { return x[i]; }
     __device__ __forceinline__ float max_with(float m) const { return fmaxf(fmaxf(m, fmaxf(x[0], x[1])), fmaxf(x[2], x[3])); }
@@ -144,6 +152,7 @@ template <> struct Vec<false> {
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const __half2*>(&w[i]);
     }
+    __device__ __forceinline__ void clear() { h[0] = h[1] = h[2] = h[3] = __half2half2(__ushort_as_half(0xfc00)); }
     __device__ __forceinline__ f2 pair(int i) const { const float2 v = __half22float2(h[i]); return pack2(v.x, v.y); }
     __device__ __forceinline__ float at(int i) const { return (i & 1) ? __high2float(h[i >> 1]) : __low2float(h[i >> 1]); }
     __device__ __forceinline__ float max_with(float m) const
@@ -225,32 +234,32 @@ __device__ __forceinline__ unsigned long long merge_lists(unsigned long long a, 
     return v;
 }
 
+template <int WARPS>
 struct Shared {
     unsigned long long keys[kKeys];             // first CTA: keys that reach the threshold, or the CTAs' lists
-    unsigned long long lists[kWarps][32];
-    Part parts[kWarps], of_cta[kMaxCluster];
-    float max1[kMaxCluster * kWarps];           // of every warp of the cluster
-    float max2[kWarps];                         // second largest thread of this CTA's warps
-    int before[kWarps], before_cta[kMaxCluster];
-    int cand[kThreads];
-    unsigned n_keys, n_cand, flooded;
+    unsigned long long lists[WARPS][32];
+    float m[kMaxCluster * WARPS], z[kMaxCluster * WARPS], t[kMaxCluster * WARPS];   // first CTA: the parts of the cluster's warps
+    int before[kMaxCluster * WARPS];
+    float reach[kMaxCluster * WARPS];           // what a group of logits of every warp of the cluster reaches
+    int cand[WARPS][32];
+    unsigned n_keys, flooded;
 };
 
-// U vectors of a thread in flight.  The walk takes 32 logits at a time of either type.
-template <bool F32, bool RANK>
-__global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobParams p)
+// The walk takes 4 vectors of a thread at a time, while the next 4 are on their way.
+template <bool F32, bool RANK, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const LogprobParams p)
 {
     using V = Vec<F32>;
     using E = typename std::conditional<F32, float, __half>::type;
-    constexpr int U = 32 / V::N;
-    __shared__ Shared sh;
+    constexpr int U = 4, kThreads = WARPS * 32, kStep = kThreads * U;
+    __shared__ Shared<WARPS> sh;
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int cta, ctas;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
-    if (tid == 0) sh.n_keys = sh.n_cand = sh.flooded = 0;
-    if (ctas > 1) cluster_arrive();             // every CTA has started, and cleared its counters, when the wait below ends
+    if (tid == 0) sh.n_keys = sh.flooded = 0;
+    cluster_arrive();                           // every CTA has started, and cleared its counters, when the wait below ends
     pdl_wait();
 
     const size_t r = blockIdx.x / ctas;
@@ -260,6 +269,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobParams p)
     const int nvec = (p.vocab - head) / V::N, tail = p.vocab - head - nvec * V::N;
     const uint4* vecs = reinterpret_cast<const uint4*>(row + head * sizeof(E));
     const int v0 = int((long long) nvec * cta / ctas), v1 = int((long long) nvec * (cta + 1) / ctas);
+    V v[U], next[U];
+    auto fetch = [&](V (&to)[U], int start) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = start + tid + u * kThreads;
+            if (i < v1) to[u].load(vecs + i);
+            else to[u].clear();   // adds nothing: below every threshold but that of a masked token, which is taken back
+        }
+    };
+    fetch(v, v0);
 
     int token = -1, before = 0, token_vec = 0;
     bool real = false;
@@ -277,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobParams p)
     }
 
     // the first CTA's threads 0..head-1 and 16..16+tail-1 begin with a single logit
-    Part own{-INFINITY, 0.0, 0.0};
+    float m = -INFINITY, z = 0.f, z_low = 0.f, t = 0.f;   // z + z_low: the sum with the maximum's 1
     int single = -1;
     if (cta == 0) {
         if (tid < head) single = tid;
@@ -285,162 +304,142 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobParams p)
     }
     if (single >= 0) {
         const float x = value_at<F32>(row, single);
-        own.m = x != x ? -INFINITY : x;
-        own.z = x != x ? NAN : (x > -INFINITY ? 1.0 : 0.0);
+        m = x != x ? -INFINITY : x;
+        z = x != x || x == INFINITY ? NAN : (x > -INFINITY ? 1.f : 0.f);
         if (RANK) before += order_key(x, single) > token_key;
     }
     // equal logits before the token in its own vector (the walk counts the larger ones there)
-    if (RANK && real && cta == 0 && tid >= 32 && tid < 32 + V::N && token_vec >= 0) {
+    if (RANK && real && cta == 0 && tid >= 32 && tid < 32 + V::N && token_vec >= 0 && token_vec < nvec) {
         const int i = head + token_vec * V::N + tid - 32;
-        if (i < token && token_vec < nvec) before += value_at<F32>(row, i) == key_value(token_key);
+        if (i < token) before += value_at<F32>(row, i) == key_value(token_key);
     }
 
-    for (int base = v0 + tid; base < v1; base += kThreads * U) {
-        V v[U];
+    for (int start = v0; start < v1; start += kStep) {
+        if (start + kStep < v1) fetch(next, start + kStep);
         float g = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = base + u * kThreads;
-            if (i < v1) v[u].load(vecs + i);
-            else {   // adds nothing: below every threshold but that of a masked token, which is taken back
-                uint4 none = F32 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u) : make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
-                memcpy(&v[u], &none, 16);
-            }
-        }
-#pragma unroll
         for (int u = 0; u < U; ++u) g = v[u].max_with(g);
-        if (g > own.m) own = brought_to(own, g, p.scale2);
-        const float ref = own.m > -INFINITY ? own.m : 0.f;
+        if (g > m) {
+            if (m > -INFINITY) {
+                const float d = (m - g) * p.scale2, f = ex2(d);
+                t = f != 0.f ? (t + d * (z + z_low)) * f : z * f;
+                z *= f;
+                z_low *= f;
+            }
+            m = g;
+        }
+        const float ref = m > -INFINITY ? m : 0.f;
         const f2 nref = pack2(-ref, -ref), sc = pack2(p.scale2, p.scale2);
-        f2 z[U], t[U];
+        f2 zs[U], ts[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             f2 e[V::N / 2];
 #pragma unroll
             for (int i = 0; i < V::N / 2; ++i) {
-                const f2 y2 = mul2(add2(v[u].pair(i), nref), sc);
                 float a, b;
-                unpack2(y2, a, b);
-                a = a < -200.f ? -200.f : a;      // a masked logit: 2^y is 0 either way, 0 * -inf is not (NaN stays)
-                b = b < -200.f ? -200.f : b;
+                unpack2(mul2(add2(v[u].pair(i), nref), sc), a, b);
+                a = max_nan(a, -200.f);      // a masked logit: 2^y is 0 either way, 0 * -inf is not
+                b = max_nan(b, -200.f);
                 e[i] = pack2(ex2(a), ex2(b));
-                t[u] = i == 0 ? mul2(e[i], pack2(a, b)) : fma2(e[i], pack2(a, b), t[u]);
+                ts[u] = i == 0 ? mul2(e[i], pack2(a, b)) : fma2(e[i], pack2(a, b), ts[u]);
             }
-            z[u] = add2(e[0], e[1]);
-            if constexpr (V::N == 8) z[u] = add2(z[u], add2(e[2], e[3]));
+            zs[u] = add2(e[0], e[1]);
+            if constexpr (V::N == 8) zs[u] = add2(zs[u], add2(e[2], e[3]));
         }
-#pragma unroll
-        for (int w = U / 2; w >= 1; w >>= 1)
-#pragma unroll
-            for (int u = 0; u < w; ++u) { z[u] = add2(z[u], z[u + w]); t[u] = add2(t[u], t[u + w]); }
+        const f2 z4 = add2(add2(zs[0], zs[1]), add2(zs[2], zs[3])), t4 = add2(add2(ts[0], ts[1]), add2(ts[2], ts[3]));
         float za, zb, ta, tb;
-        unpack2(z[0], za, zb);
-        unpack2(t[0], ta, tb);
-        own.z += double(za) + double(zb);
-        own.t += double(ta) + double(tb);
+        unpack2(z4, za, zb);
+        unpack2(t4, ta, tb);
+        za += zb;
+        const float sum = z + za, part = sum - z;   // two-sum: z_low takes what sum rounds off
+        z_low += (z - (sum - part)) + (za - part);
+        z = sum;
+        t += ta + tb;
         if (RANK && real) {
             E thr[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) thr[u] = base + u * kThreads < token_vec ? at : over;
+            for (int u = 0; u < U; ++u) thr[u] = start + tid + u * kThreads < token_vec ? at : over;
             before += count_ge(v, thr);
             if (token_key >> 32 == 0x007fffffu)   // a masked token: the vectors behind the end counted as equal
-                for (int u = 0; u < U; ++u)
-                    if (base + u * kThreads >= v1 && base + u * kThreads < token_vec) before -= V::N;
+                for (int u = 0; u < U; ++u) {
+                    const int i = start + tid + u * kThreads;
+                    if (i >= v1 && i < token_vec) before -= V::N;
+                }
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = next[u];
     }
 
-    // ---- join: warps, CTA, cluster
-    const float mine = own.m;
-    Part part = joined<32>(own, p.scale2);
+    // ---- join: the warps leave their parts with the first CTA, and with every CTA what they reach
+    const Part own = joined(Part{m, m > -INFINITY ? (z - 1.f) + z_low : z, t}, p.scale2);
     if (RANK) before = __reduce_add_sync(dq::kFull, before);
-    if (p.top_n > kWarps && ctas == 1) {
-        const unsigned first = __ffs(__ballot_sync(dq::kFull, mine == part.m)) - 1;   // (a warp without a maximum: -inf == -inf)
-        float other = lane == int(first) ? -INFINITY : mine;
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) other = fmaxf(other, __shfl_xor_sync(dq::kFull, other, off));
-        if (lane == 0) sh.max2[warp] = other;
-    }
-    if (lane == 0) {
-        sh.parts[warp] = part;
-        sh.before[warp] = before;
-        if (ctas == 1) sh.max1[warp] = part.m;
-    }
-    if (ctas > 1) cluster_wait();
-    __syncthreads();
-    if (ctas > 1 && p.top_n > 0 && tid < ctas * kWarps)
-        peer_store(peer_addr(&sh.max1[cta * kWarps + (tid & (kWarps - 1))], tid / kWarps), __float_as_uint(sh.parts[tid & (kWarps - 1)].m));
-    if (warp == 0) {
-        part = lane < kWarps ? sh.parts[lane] : Part{-INFINITY, 0.0, 0.0};
-        part = joined<32>(part, p.scale2);
-        const int b = RANK ? __reduce_add_sync(dq::kFull, lane < kWarps ? sh.before[lane] : 0) : 0;
-        if (ctas == 1) {
-            if (lane == 0) { sh.of_cta[0] = part; sh.before_cta[0] = b; }
-        } else if (lane == 0) {
-            peer_store(peer_addr(&sh.of_cta[cta].m, 0), __float_as_uint(part.m));
-            peer_store(peer_addr(&sh.of_cta[cta].z, 0), (unsigned long long) __double_as_longlong(part.z));
-            peer_store(peer_addr(&sh.of_cta[cta].t, 0), (unsigned long long) __double_as_longlong(part.t));
-            peer_store(peer_addr(&sh.before_cta[cta], 0), unsigned(b));
+    const int warps = ctas * WARPS, me = cta * WARPS + warp;
+    // at least n groups of logits: whole warps, or if there are fewer, the k largest threads of each
+    float reach = own.m;
+    if (p.top_n > warps) {
+        const int k = (p.top_n + warps - 1) / warps;
+        float rest = m;
+        for (int i = 1; i < k; ++i) {
+            if (lane == __ffs(__ballot_sync(dq::kFull, rest == reach)) - 1) rest = -INFINITY;
+            reach = redux_max(rest);
         }
     }
-    if (ctas > 1) { cluster_arrive(); cluster_wait(); }
-    else __syncthreads();
+    cluster_wait();
+    if (lane == 0) {
+        peer_store(peer_addr(&sh.m[me], 0), __float_as_uint(own.m));
+        peer_store(peer_addr(&sh.z[me], 0), __float_as_uint(own.z));
+        peer_store(peer_addr(&sh.t[me], 0), __float_as_uint(own.t));
+        peer_store(peer_addr(&sh.before[me], 0), unsigned(before));
+    }
+    if (p.top_n > 0 && lane < ctas) peer_store(peer_addr(&sh.reach[me], lane), __float_as_uint(reach));
+    cluster_arrive();
+    cluster_wait();
 
     // ---- the candidates for the n best
     if (p.top_n > 0) {
-        // at least n groups of warps; tau = the smallest of their maxima
         int groups = 1;
         while (groups < p.top_n) groups <<= 1;
-        const int warps = ctas * kWarps;
+        // tau: the least of what the groups reach
         float tau = -INFINITY;
-        if (groups <= warps) {
-            for (int i = lane; i < warps; i += 32) tau = fmaxf(tau, sh.max1[i]);
-            if (warps < 32) tau = __shfl_sync(dq::kFull, tau, lane & (kWarps - 1));   // one CTA: 16 warps
+        for (int i = lane; i < warps; i += 32) tau = fmaxf(tau, sh.reach[i]);
+        if (warps < 32) tau = __shfl_sync(dq::kFull, tau, lane & (warps - 1));
+        if (p.top_n <= warps)
             for (int off = groups; off < 32; off <<= 1) tau = fmaxf(tau, __shfl_xor_sync(dq::kFull, tau, off));
-        } else {
-            tau = sh.max2[lane & (kWarps - 1)];   // one CTA, n > 16: two threads of every warp
-        }
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) tau = fminf(tau, __shfl_xor_sync(dq::kFull, tau, off));
+        tau = redux_min(tau);
 
         const int per_thread = (v1 - v0 + kThreads - 1) / kThreads;
-        const uint32_t keys0 = ctas > 1 ? peer_addr(sh.keys, 0) : smem_addr(sh.keys), n0 = ctas > 1 ? peer_addr(&sh.n_keys, 0) : smem_addr(&sh.n_keys);
+        const uint32_t keys0 = peer_addr(sh.keys, 0), n0 = peer_addr(&sh.n_keys, 0);
+        auto flood = [&] { for (int i = 0; i < ctas; ++i) peer_store(peer_addr(&sh.flooded, i), 1u); };
         auto push = [&](float x, int i) {
             const unsigned at_key = peer_add(n0, 1u);
             if (at_key < unsigned(kKeys)) peer_store(keys0 + at_key * 8, order_key(x, i));
-            else sh.flooded = 1;
+            else flood();
         };
         if (tau > -INFINITY) {
-            const unsigned has = __ballot_sync(dq::kFull, mine >= tau);
-            unsigned at_cand = 0;
-            if (lane == 0 && has) at_cand = atomicAdd(&sh.n_cand, __popc(has));
-            at_cand = __shfl_sync(dq::kFull, at_cand, 0) + __popc(has & ((1u << lane) - 1));
-            if (mine >= tau) sh.cand[at_cand] = tid;
-            if (single >= 0) {
-                const float x = value_at<F32>(row, single);
-                if (x >= tau) push(x, single);
-            }
-            __syncthreads();
-            const int n_cand = int(sh.n_cand);
-            if (n_cand <= kThreads / 2) {
-                for (int k = tid; k < n_cand * per_thread; k += kThreads) {
-                    const int i = v0 + sh.cand[k / per_thread] + (k % per_thread) * kThreads;
+            const unsigned has = __ballot_sync(dq::kFull, m >= tau);
+            const int n_cand = __popc(has);
+            if (m >= tau) sh.cand[warp][__popc(has & ((1u << lane) - 1))] = tid;
+            __syncwarp();
+            if (n_cand * per_thread <= 16 * per_thread + 32) {
+                for (int k = lane; k < n_cand * per_thread; k += 32) {
+                    const int i = v0 + sh.cand[warp][k / per_thread] + (k % per_thread) * kThreads;
                     if (i < v1) {
-                        V v;
-                        v.load(vecs + i);
-                        if (v.max_with(-INFINITY) >= tau) {
+                        V w;
+                        w.load(vecs + i);
+                        if (w.max_with(-INFINITY) >= tau) {
 #pragma unroll
                             for (int e = 0; e < V::N; ++e)
-                                if (v.at(e) >= tau) push(v.at(e), head + i * V::N + e);
+                                if (w.at(e) >= tau) push(w.at(e), head + i * V::N + e);
                         }
                     }
                 }
-            } else if (tid == 0) sh.flooded = 1;
-            __syncthreads();
-            if (ctas > 1) {
-                if (tid < ctas && sh.flooded) peer_store(peer_addr(&sh.flooded, tid), 1u);
-                cluster_arrive();
-                cluster_wait();
-            }
+                if (single >= 0) {
+                    const float x = value_at<F32>(row, single);
+                    if (x >= tau) push(x, single);
+                }
+            } else if (lane == 0) flood();
+            cluster_arrive();
+            cluster_wait();
         }
         if (tau == -INFINITY || sh.flooded) {
             // the whole part again, 32 sorted keys a warp
@@ -448,13 +447,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobParams p)
             offer_keys(list, single >= 0 ? order_key(value_at<F32>(row, single), single) : 0, p.top_n);
             for (int base = v0 + warp * 32; base < v1; base += kThreads) {
                 const int i = base + lane;
-                V v;
-                if (i < v1) v.load(vecs + i);
+                V w;
+                if (i < v1) w.load(vecs + i);
 #pragma unroll
-                for (int e = 0; e < V::N; ++e) offer_keys(list, i < v1 && !(v.at(e) < tau) ? order_key(v.at(e), head + i * V::N + e) : 0, p.top_n);
+                for (int e = 0; e < V::N; ++e) offer_keys(list, i < v1 && !(w.at(e) < tau) ? order_key(w.at(e), head + i * V::N + e) : 0, p.top_n);
             }
             sh.lists[warp][lane] = list;
-            for (int w = kWarps / 2; w >= 1; w >>= 1) {
+            for (int w = WARPS / 2; w >= 1; w >>= 1) {
                 __syncthreads();
                 if (warp < w) {
                     list = merge_lists(list, sh.lists[warp + w][lane]);
@@ -465,42 +464,54 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobParams p)
                 if (lane < p.top_n) peer_store(keys0 + (cta * p.top_n + lane) * 8, list);
                 if (cta == 0 && lane == 0) sh.n_keys = ctas * p.top_n;
             }
-            if (ctas > 1) { cluster_arrive(); cluster_wait(); }
-            else __syncthreads();
+            cluster_arrive();
+            cluster_wait();
         }
     }
     if (cta != 0) return;
 
     // ---- the first CTA writes the row's answers
-    part = joined<32>(lane < ctas ? sh.of_cta[lane] : Part{-INFINITY, 0.0, 0.0}, p.scale2);
-    const bool none = part.m == -INFINITY && part.z == 0.0;   // masked altogether
-    const float m = part.m, lnz = log1pf(float(part.z - 1.0));
+    Part all{-INFINITY, 0.f, 0.f};
+    for (int i = lane; i < warps; i += 32) all = joined(all, Part{sh.m[i], sh.z[i], sh.t[i]}, p.scale2);
+    all = joined(all, p.scale2);
+    const bool none = all.m == -INFINITY && all.z == 0.f;   // masked altogether
+    const float lnz = log1pf(all.z);
     // the difference is taken before the scale: a row of the type's lowest value would overflow the product
-    auto logprob_of = [&](float x) { return none ? -INFINITY : (x - m) * p.inv_temp - lnz; };
+    auto logprob_of = [&](float x) { return none ? -INFINITY : (x - all.m) * p.inv_temp - lnz; };
     if (warp == 0) {
-        const int rank = RANK ? __reduce_add_sync(dq::kFull, lane < ctas ? sh.before_cta[lane] : 0) : 0;
+        int rank = 0;
+        if (RANK) {
+            for (int i = lane; i < warps; i += 32) rank += sh.before[i];
+            rank = __reduce_add_sync(dq::kFull, rank);
+        }
         if (lane == 0) {
             if (RANK && p.logprob) p.logprob[r] = real ? logprob_of(key_value(token_key)) : 0.f;
             if (RANK && p.rank) p.rank[r] = real && token_key >> 32 ? rank : -1;
-            if (p.entropy) p.entropy[r] = none ? 0.f : lnz - float(part.t / part.z) * kLn2;
+            if (p.entropy) p.entropy[r] = none ? 0.f : lnz - all.t / (1.f + all.z) * kLn2;
         }
     }
-    const int n_keys = p.top_n > 0 ? int(sh.n_keys) : 0;
-    if (tid < n_keys) {
-        const unsigned long long key = sh.keys[tid];
-        int place = 0;
-        for (int i = 0; i < n_keys; ++i) place += sh.keys[i] > key;
-        if (place < p.top_n && key != 0) {
-            p.top_idx[r * p.top_n + place] = int(0xffffffffu - unsigned(key));
-            p.top_logprob[r * p.top_n + place] = logprob_of(key_value(key));
+    if (p.top_n > 0) {   // four threads count the keys before one
+        const int n_keys = int(sh.n_keys), part = tid & 3;
+        for (int base = 0; base < n_keys; base += kThreads / 4) {
+            const int k = base + (tid >> 2);
+            const unsigned long long key = k < n_keys ? sh.keys[k] : 0;
+            int place = 0;
+#pragma unroll 4
+            for (int i = part; i < n_keys; i += 4) place += sh.keys[i] > key;
+            place += __shfl_xor_sync(dq::kFull, place, 1);
+            place += __shfl_xor_sync(dq::kFull, place, 2);
+            if (part == 0 && key != 0 && place < p.top_n) {
+                p.top_idx[r * p.top_n + place] = int(0xffffffffu - unsigned(key));
+                p.top_logprob[r * p.top_n + place] = logprob_of(key_value(key));
+            }
         }
     }
 }
 
-template <bool F32, bool RANK>
+template <bool F32, bool RANK, int WARPS>
 void launch(const LogprobParams& p, int ctas, cudaStream_t st)
 {
-    auto kern = k_logprobs<F32, RANK>;
+    auto kern = k_logprobs<F32, RANK, WARPS>;
     static bool set[kMaxDevices] = {};
     const int dev = current_device();
     if (!set[dev]) {
@@ -509,7 +520,7 @@ void launch(const LogprobParams& p, int ctas, cudaStream_t st)
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(p.rows) * unsigned(ctas));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(WARPS * 32);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -521,19 +532,20 @@ void launch(const LogprobParams& p, int ctas, cudaStream_t st)
     cfg.numAttrs = 2;
     cuda_ok(cudaLaunchKernelEx(&cfg, kern, p), "logprobs launch");
 }
-
-// CTAs a row is split over.
-int row_ctas(int rows, long long row_bytes)
+template <bool F32, bool RANK>
+void launch(const LogprobParams& p, int ctas, int warps, cudaStream_t st)
 {
-    int best = 1;
-    double least = 0.0;
-    for (int s = 1; s <= kMaxCluster; s *= 2) {
-        const long long slots = 296 / s;                       // clusters that run at once (two CTAs an SM)
-        const long long waves = (rows + slots - 1) / slots;
-        const double t = double(waves) * (3.0 + double(row_bytes) / s / 22e3);   // us: fixed part, then some 22 GB/s... a CTA's share
-        if (s == 1 || t < least) { best = s; least = t; }
-    }
-    return best;
+    if (warps == 4) launch<F32, RANK, 4>(p, ctas, st);
+    else if (warps == 8) launch<F32, RANK, 8>(p, ctas, st);
+    else launch<F32, RANK, 16>(p, ctas, st);
+}
+
+// CTAs a row is split over and warps of each.
+void row_split(int rows, long long row_bytes, int& ctas, int& warps)
+{
+    warps = row_bytes <= 16384 ? 4 : 16;
+    ctas = 1;
+    while (ctas < 16 && rows * ctas * 2 <= 296 && row_bytes / ctas > 32768) ctas *= 2;
 }
 
 }  // namespace
@@ -559,11 +571,12 @@ extern "C" int berth_ops_logprobs(const void* logits, int logits_fp32, int64_t r
         if (rows > (1 << 26)) throw std::runtime_error("logprobs: rows must be at most 2^26");
         const LogprobParams p{logits, row_stride, tokens, logprob, rank, entropy, top_idx, top_logprob, top_n, rows, vocab, inv_temp, inv_temp * kLog2e};
         const bool f32 = logits_fp32 != 0, ranks = logprob || rank;
-        const int ctas = row_ctas(rows, (long long) vocab * (f32 ? 4 : 2));
+        int ctas, warps;
+        row_split(rows, (long long) vocab * (f32 ? 4 : 2), ctas, warps);
         cudaStream_t cs = (cudaStream_t) stream;
-        if (f32) ranks ? launch<true, true>(p, ctas, cs) : launch<true, false>(p, ctas, cs);
-        else ranks ? launch<false, true>(p, ctas, cs) : launch<false, false>(p, ctas, cs);
-        st.launch = std::string("k_logprobs<") + (f32 ? "float" : "half") + (ranks ? ",rank" : "") + "> block=" + std::to_string(kThreads) + " grid=" +
+        if (f32) ranks ? launch<true, true>(p, ctas, warps, cs) : launch<true, false>(p, ctas, warps, cs);
+        else ranks ? launch<false, true>(p, ctas, warps, cs) : launch<false, false>(p, ctas, warps, cs);
+        st.launch = std::string("k_logprobs<") + (f32 ? "float" : "half") + (ranks ? ",rank" : "") + "> block=" + std::to_string(warps * 32) + " grid=" +
                     std::to_string(rows) + "x" + std::to_string(ctas) + " cluster=" + std::to_string(ctas);
     });
 }
