@@ -8,14 +8,15 @@
 //
 // The n best come out of the walk's by-product, the threads' maxima.  The cluster's warps fall into at least n groups (or
 // give their k largest threads each, where there are fewer warps than n); the smallest of the groups' maxima is a value that n logits reach, and few more do, all of them in threads whose maximum
-// reaches it.  Only those threads' vectors are read again (from L2, a few percent of the row), what reaches the value goes to
-// the first CTA's shared memory, and each finds its place by counting the larger ones.  Rows where too many reach it (equal
+// reaches it.  Only those threads' vectors are read again, and of those only the steps of the walk in which the warp reached
+// it (well below a percent of the row), what reaches the value goes to the first CTA's shared memory, and each finds its place by counting the larger ones.  Rows where too many reach it (equal
 // logits, a mask that leaves fewer than n) are scanned once more with a sorted list of 32 per warp instead.
 #include "exl3_decode.cuh"
 #include "../../include/berth_b200.h"
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace berth {
 namespace {
@@ -60,6 +61,8 @@ __device__ __forceinline__ float key_value(unsigned long long key)
 }
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 
 // Two fp32 lanes of one 64-bit register (one instruction for both).
 struct f2 { unsigned long long v; };
@@ -138,9 +141,9 @@ template <> struct Vec<true> {
         x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
     }
     __device__ __forceinline__ void clear() { x[0] = x[1] = x[2] = x[3] = -INFINITY; }
-    __device__ __forceinline__ f2 pair(int i) const { return pack2(x[2 * i], x[2 * i + 1]); }
+    __device__ __forceinline__ f2 pair_plus(int i, float c) const { return add2(pack2(x[2 * i], x[2 * i + 1]), pack2(c, c)); }
     __device__ __forceinline__ float at(int i) const { return x[i]; }
-    __device__ __forceinline__ float max_with(float m) const { return fmaxf(fmaxf(m, fmaxf(x[0], x[1])), fmaxf(x[2], x[3])); }
+    __device__ __forceinline__ float max_with(float m) const { return max3(max3(m, x[0], x[1]), x[2], x[3]); }
 };
 template <> struct Vec<false> {
     static constexpr int N = 8;
@@ -153,7 +156,13 @@ template <> struct Vec<false> {
         for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const __half2*>(&w[i]);
     }
     __device__ __forceinline__ void clear() { h[0] = h[1] = h[2] = h[3] = __half2half2(__ushort_as_half(0xfc00)); }
-    __device__ __forceinline__ f2 pair(int i) const { const float2 v = __half22float2(h[i]); return pack2(v.x, v.y); }
+    __device__ __forceinline__ f2 pair_plus(int i, float c) const   // converted and added in one instruction
+    {
+        float a, b;
+        asm("add.f32.f16 %0, %1, %2;" : "=f"(a) : "h"(__half_as_ushort(__low2half(h[i]))), "f"(c));
+        asm("add.f32.f16 %0, %1, %2;" : "=f"(b) : "h"(__half_as_ushort(__high2half(h[i]))), "f"(c));
+        return pack2(a, b);
+    }
     __device__ __forceinline__ float at(int i) const { return (i & 1) ? __high2float(h[i >> 1]) : __low2float(h[i >> 1]); }
     __device__ __forceinline__ float max_with(float m) const
     {
@@ -259,7 +268,11 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
     if (tid == 0) sh.n_keys = sh.flooded = 0;
-    cluster_arrive();                           // every CTA has started, and cleared its counters, when the wait below ends
+    if (ctas > 1) cluster_arrive();             // every CTA has started, and cleared its counters, when the wait below ends
+    auto sync_all = [&] {
+        if (ctas > 1) { cluster_arrive(); cluster_wait(); }
+        else __syncthreads();
+    };
     pdl_wait();
 
     const size_t r = blockIdx.x / ctas;
@@ -271,11 +284,16 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
     const int v0 = int((long long) nvec * cta / ctas), v1 = int((long long) nvec * (cta + 1) / ctas);
     V v[U], next[U];
     auto fetch = [&](V (&to)[U], int start) {
+        const uint4* from = vecs + start + tid;
+        if (start + kStep <= v1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = start + tid + u * kThreads;
-            if (i < v1) to[u].load(vecs + i);
-            else to[u].clear();   // adds nothing: below every threshold but that of a masked token, which is taken back
+            for (int u = 0; u < U; ++u) to[u].load(from + u * kThreads);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                to[u].clear();   // adds nothing: below every threshold but that of a masked token, which is taken back
+                if (start + tid + u * kThreads < v1) to[u].load(from + u * kThreads);
+            }
         }
     };
     fetch(v, v0);
@@ -294,6 +312,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
             token_vec = token < head ? -1 : (token - head) / V::N;
         }
     }
+    const float least = real ? (F32 ? float(at) : __half2float(at)) : INFINITY;   // (no token, or a NaN: nothing is counted)
 
     // the first CTA's threads 0..head-1 and 16..16+tail-1 begin with a single logit
     float m = -INFINITY, z = 0.f, z_low = 0.f, t = 0.f;   // z + z_low: the sum with the maximum's 1
@@ -314,11 +333,15 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
         if (i < token) before += value_at<F32>(row, i) == key_value(token_key);
     }
 
-    for (int start = v0; start < v1; start += kStep) {
-        if (start + kStep < v1) fetch(next, start + kStep);
+    float step_max = -INFINITY;   // lane i: the warp's maximum in the steps i, i + 32, ..
+    auto take = [&](int start, int step) {
         float g = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u) g = v[u].max_with(g);
+        if (p.top_n > 0) {
+            const float w = redux_max(g);
+            if (lane == (step & 31)) step_max = fmaxf(step_max, w);
+        }
         if (g > m) {
             if (m > -INFINITY) {
                 const float d = (m - g) * p.scale2, f = ex2(d);
@@ -328,8 +351,8 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
             }
             m = g;
         }
-        const float ref = m > -INFINITY ? m : 0.f;
-        const f2 nref = pack2(-ref, -ref), sc = pack2(p.scale2, p.scale2);
+        const float nref = m > -INFINITY ? -m : 0.f;
+        const f2 sc = pack2(p.scale2, p.scale2);
         f2 zs[U], ts[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -337,8 +360,8 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
 #pragma unroll
             for (int i = 0; i < V::N / 2; ++i) {
                 float a, b;
-                unpack2(mul2(add2(v[u].pair(i), nref), sc), a, b);
-                a = max_nan(a, -200.f);      // a masked logit: 2^y is 0 either way, 0 * -inf is not
+                unpack2(mul2(v[u].pair_plus(i, nref), sc), a, b);
+                a = max_nan(a, -200.f);   // a masked logit: 2^y is 0 either way, 0 * -inf is not
                 b = max_nan(b, -200.f);
                 e[i] = pack2(ex2(a), ex2(b));
                 ts[u] = i == 0 ? mul2(e[i], pack2(a, b)) : fma2(e[i], pack2(a, b), ts[u]);
@@ -355,7 +378,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
         z_low += (z - (sum - part)) + (za - part);
         z = sum;
         t += ta + tb;
-        if (RANK && real) {
+        if (RANK && g >= least) {               // most tokens are likely ones: few vectors reach them
             E thr[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) thr[u] = start + tid + u * kThreads < token_vec ? at : over;
@@ -366,6 +389,11 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
                     if (i >= v1 && i < token_vec) before -= V::N;
                 }
         }
+    };
+    int step = 0;
+    for (int start = v0; start < v1; start += kStep, ++step) {
+        if (start + kStep < v1) fetch(next, start + kStep);
+        take(start, step);
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = next[u];
     }
@@ -384,7 +412,8 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
             reach = redux_max(rest);
         }
     }
-    cluster_wait();
+    if (ctas > 1) cluster_wait();
+    else __syncthreads();
     if (lane == 0) {
         peer_store(peer_addr(&sh.m[me], 0), __float_as_uint(own.m));
         peer_store(peer_addr(&sh.z[me], 0), __float_as_uint(own.z));
@@ -392,8 +421,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
         peer_store(peer_addr(&sh.before[me], 0), unsigned(before));
     }
     if (p.top_n > 0 && lane < ctas) peer_store(peer_addr(&sh.reach[me], lane), __float_as_uint(reach));
-    cluster_arrive();
-    cluster_wait();
+    sync_all();
 
     // ---- the candidates for the n best
     if (p.top_n > 0) {
@@ -407,7 +435,6 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
             for (int off = groups; off < 32; off <<= 1) tau = fmaxf(tau, __shfl_xor_sync(dq::kFull, tau, off));
         tau = redux_min(tau);
 
-        const int per_thread = (v1 - v0 + kThreads - 1) / kThreads;
         const uint32_t keys0 = peer_addr(sh.keys, 0), n0 = peer_addr(&sh.n_keys, 0);
         auto flood = [&] { for (int i = 0; i < ctas; ++i) peer_store(peer_addr(&sh.flooded, i), 1u); };
         auto push = [&](float x, int i) {
@@ -420,26 +447,27 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
             const int n_cand = __popc(has);
             if (m >= tau) sh.cand[warp][__popc(has & ((1u << lane) - 1))] = tid;
             __syncwarp();
-            if (n_cand * per_thread <= 16 * per_thread + 32) {
-                for (int k = lane; k < n_cand * per_thread; k += 32) {
-                    const int i = v0 + sh.cand[warp][k / per_thread] + (k % per_thread) * kThreads;
-                    if (i < v1) {
-                        V w;
-                        w.load(vecs + i);
-                        if (w.max_with(-INFINITY) >= tau) {
+            if (n_cand <= 16 || step <= 1) {
+                // in the steps in which the warp reached tau, eight threads' four vectors at a time
+                for (unsigned steps = __ballot_sync(dq::kFull, step_max >= tau); steps; steps &= steps - 1)
+                    for (int j = __ffs(steps) - 1; j < step; j += 32)
+                        for (int c = lane >> 2; c < n_cand; c += 8) {
+                            const int i = v0 + j * kStep + sh.cand[warp][c] + (lane & 3) * kThreads;
+                            if (i >= v1) continue;
+                            V w;
+                            w.load(vecs + i);
+                            if (w.max_with(-INFINITY) >= tau) {
 #pragma unroll
-                            for (int e = 0; e < V::N; ++e)
-                                if (w.at(e) >= tau) push(w.at(e), head + i * V::N + e);
+                                for (int e = 0; e < V::N; ++e)
+                                    if (w.at(e) >= tau) push(w.at(e), head + i * V::N + e);
+                            }
                         }
-                    }
-                }
                 if (single >= 0) {
                     const float x = value_at<F32>(row, single);
                     if (x >= tau) push(x, single);
                 }
             } else if (lane == 0) flood();
-            cluster_arrive();
-            cluster_wait();
+            sync_all();
         }
         if (tau == -INFINITY || sh.flooded) {
             // the whole part again, 32 sorted keys a warp
@@ -464,8 +492,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
                 if (lane < p.top_n) peer_store(keys0 + (cta * p.top_n + lane) * 8, list);
                 if (cta == 0 && lane == 0) sh.n_keys = ctas * p.top_n;
             }
-            cluster_arrive();
-            cluster_wait();
+            sync_all();
         }
     }
     if (cta != 0) return;
