@@ -25,6 +25,8 @@ constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 constexpr int kMaxTop = 32, kMaxCluster = 16, kKeys = 512;
 static_assert(kMaxCluster * kMaxTop <= kKeys, "the lists of a cluster share the key buffer");
 
+constexpr int kUnroll = 4, kRingBytes = 2 * kUnroll * 32 * 16;   // vectors of a thread in a step; the ring of a warp
+
 struct LogprobParams {
     const void* logits;
     long long ld;
@@ -109,25 +111,31 @@ __device__ __forceinline__ Part beside(Part p, float m, float scale2)
     }
     return p;
 }
-__device__ __forceinline__ Part joined(const Part& a, const Part& b, float scale2)
+// The N parts of each of the warp's lanes as one, in every lane (the order of the sums is fixed).
+template <int N>
+__device__ __forceinline__ Part joined(const Part (&p)[N], float scale2)
 {
-    const bool first = a.m >= b.m;
-    const Part &h = first ? a : b, o = beside(first ? b : a, h.m, scale2);
-    return Part{h.m, h.z + o.z, h.t + o.t};
-}
-// The parts of the warp's lanes as one, in every lane (the order of the sums is fixed).
-__device__ __forceinline__ Part joined(Part p, float scale2)
-{
-    const float m = redux_max(p.m);
-    const int holder = __ffs(__ballot_sync(dq::kFull, p.m == m)) - 1;
-    if (int(threadIdx.x & 31) != holder) p = beside(p, m, scale2);
+    float m = p[0].m;
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, p[i].m);
+    const float mine = m;
+    m = redux_max(m);
+    bool holds = int(threadIdx.x & 31) == __ffs(__ballot_sync(dq::kFull, mine == m)) - 1;   // the first part with the maximum keeps its 1 out
+    Part all{m, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool keeps = holds && p[i].m == m;
+        holds = holds && !keeps;
+        const Part o = keeps ? p[i] : beside(p[i], m, scale2);
+        all.z += o.z;
+        all.t += o.t;
+    }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) {
-        p.z += __shfl_xor_sync(dq::kFull, p.z, off);
-        p.t += __shfl_xor_sync(dq::kFull, p.t, off);
+        all.z += __shfl_xor_sync(dq::kFull, all.z, off);
+        all.t += __shfl_xor_sync(dq::kFull, all.t, off);
     }
-    p.m = m;
-    return p;
+    return all;
 }
 
 // 16 bytes of a row: 8 fp16 or 4 fp32.
@@ -137,7 +145,10 @@ template <> struct Vec<true> {
     float x[4];
     __device__ __forceinline__ void load(const uint4* a)
     {
-        const uint4 v = __ldcg(a);
+        set(__ldcg(a));
+    }
+    __device__ __forceinline__ void set(const uint4& v)
+    {
         x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
     }
     __device__ __forceinline__ void clear() { x[0] = x[1] = x[2] = x[3] = -INFINITY; }
@@ -150,7 +161,10 @@ template <> struct Vec<false> {
     __half2 h[4];
     __device__ __forceinline__ void load(const uint4* a)
     {
-        const uint4 v = __ldcg(a);
+        set(__ldcg(a));
+    }
+    __device__ __forceinline__ void set(const uint4& v)
+    {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const __half2*>(&w[i]);
@@ -245,30 +259,37 @@ __device__ __forceinline__ unsigned long long merge_lists(unsigned long long a, 
 
 template <int WARPS>
 struct Shared {
-    unsigned long long keys[kKeys];             // first CTA: keys that reach the threshold, or the CTAs' lists
-    unsigned long long lists[WARPS][32];
+    unsigned long long keys[kKeys];             // first CTA: every CTA's keys that reach tau, or its list; 0 = none
+    unsigned long long lists[kKeys / 32][32];   // the warps' lists of the slow way; first CTA: the keys, one behind the other
     float m[kMaxCluster * WARPS], z[kMaxCluster * WARPS], t[kMaxCluster * WARPS];   // first CTA: the parts of the cluster's warps
     int before[kMaxCluster * WARPS];
-    float reach[kMaxCluster * WARPS];           // what a group of logits of every warp of the cluster reaches
+    alignas(16) float reach[kMaxCluster * WARPS > 32 ? kMaxCluster * WARPS : 32];   // what logits of every warp of the cluster reach
+    alignas(16) float ranked[WARPS][32];
     int cand[WARPS][32];
-    unsigned n_keys, flooded;
+    unsigned n_own, n_keys, flooded;
+    float row_m, row_lnz;
+    int none;
 };
 
-// The walk takes 4 vectors of a thread at a time, while the next 4 are on their way.
+// Vector i of the row belongs to thread i % kThreads of CTA (i / kThreads) % ctas, so that every warp sees all of the
+// vocabulary: a threshold taken from the warps' maxima then holds where the likely tokens lie close together.  The walk takes 4
+// vectors of a thread at a time, while those of the next step are on their way to shared memory.
 template <bool F32, bool RANK, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const LogprobParams p)
 {
     using V = Vec<F32>;
     using E = typename std::conditional<F32, float, __half>::type;
-    constexpr int U = 4, kThreads = WARPS * 32, kStep = kThreads * U;
+    constexpr int U = kUnroll, kThreads = WARPS * 32;
     __shared__ Shared<WARPS> sh;
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int cta, ctas;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
-    if (tid == 0) sh.n_keys = sh.flooded = 0;
-    if (ctas > 1) cluster_arrive();             // every CTA has started, and cleared its counters, when the wait below ends
+    if (cta == 0)
+        for (int i = tid; i < kKeys; i += kThreads) sh.keys[i] = 0;
+    if (tid == 0) sh.n_own = sh.n_keys = sh.flooded = 0;
+    if (ctas > 1) cluster_arrive();             // every CTA has started, and cleared its shared memory, when the wait below ends
     auto sync_all = [&] {
         if (ctas > 1) { cluster_arrive(); cluster_wait(); }
         else __syncthreads();
@@ -281,42 +302,32 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
     const int head = min(int(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(E)), p.vocab);
     const int nvec = (p.vocab - head) / V::N, tail = p.vocab - head - nvec * V::N;
     const uint4* vecs = reinterpret_cast<const uint4*>(row + head * sizeof(E));
-    const int v0 = int((long long) nvec * cta / ctas), v1 = int((long long) nvec * (cta + 1) / ctas);
-    V v[U], next[U];
-    auto fetch = [&](V (&to)[U], int start) {
-        const uint4* from = vecs + start + tid;
-        if (start + kStep <= v1) {
+    const int stride = kThreads * ctas, first = cta * kThreads + tid;   // of this thread's vectors
+    const int steps = (nvec + stride * U - 1) / (stride * U);
+    // a thread copies its vectors to places of its own in the ring and reads nothing else there: no barrier
+    extern __shared__ __align__(16) uint4 ring[];   // [2][U][kThreads]
+    const uint32_t ring_at = smem_addr(ring + tid);
+    const uint4* from = vecs + first;
+    auto request = [&](int step) {
+        const uint32_t to = ring_at + (step & 1) * (U * kThreads * 16);
+        auto copy = [&](int u) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * kThreads * 16), "l"(from + u * stride) : "memory"); };
+        if (step + 1 < steps) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) to[u].load(from + u * kThreads);
-        } else {
+            for (int u = 0; u < U; ++u) copy(u);
+        } else if (step < steps) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                to[u].clear();   // adds nothing: below every threshold but that of a masked token, which is taken back
-                if (start + tid + u * kThreads < v1) to[u].load(from + u * kThreads);
-            }
+            for (int u = 0; u < U; ++u)
+                if (first + (step * U + u) * stride < nvec) copy(u);
         }
+        from += U * stride;
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    fetch(v, v0);
-
-    int token = -1, before = 0, token_vec = 0;
-    bool real = false;
-    unsigned long long token_key = 0;
-    E at{}, over{};
-    if (RANK) {
-        token = p.tokens[r];
-        real = token >= 0 && token < p.vocab;
-        if (real) {
-            at = reinterpret_cast<const E*>(row)[token];
-            over = above(at);
-            token_key = order_key(F32 ? float(at) : __half2float(at), token);
-            token_vec = token < head ? -1 : (token - head) / V::N;
-        }
-    }
-    const float least = real ? (F32 ? float(at) : __half2float(at)) : INFINITY;   // (no token, or a NaN: nothing is counted)
+    request(0);
+    const int token = RANK ? p.tokens[r] : -1;
 
     // the first CTA's threads 0..head-1 and 16..16+tail-1 begin with a single logit
     float m = -INFINITY, z = 0.f, z_low = 0.f, t = 0.f;   // z + z_low: the sum with the maximum's 1
-    int single = -1;
+    int single = -1, before = 0, token_vec = 0;
     if (cta == 0) {
         if (tid < head) single = tid;
         else if (tid >= 16 && tid < 16 + tail) single = p.vocab - tail + tid - 16;
@@ -325,16 +336,42 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
         const float x = value_at<F32>(row, single);
         m = x != x ? -INFINITY : x;
         z = x != x || x == INFINITY ? NAN : (x > -INFINITY ? 1.f : 0.f);
-        if (RANK) before += order_key(x, single) > token_key;
     }
-    // equal logits before the token in its own vector (the walk counts the larger ones there)
-    if (RANK && real && cta == 0 && tid >= 32 && tid < 32 + V::N && token_vec >= 0 && token_vec < nvec) {
-        const int i = head + token_vec * V::N + tid - 32;
-        if (i < token) before += value_at<F32>(row, i) == key_value(token_key);
+    const bool real = token >= 0 && token < p.vocab;
+    unsigned long long token_key = 0;
+    E at{}, over{};
+    float least = INFINITY;
+    if (RANK && real) {
+        at = reinterpret_cast<const E*>(row)[token];
+        token_vec = token < head ? -1 : (token - head) / V::N;
     }
-
+    // what the count of the logits before the token needs; behind the first step's sums, which do not wait for it
+    auto look_at_token = [&] {
+        if (!RANK || !real) return;
+        over = above(at);
+        least = F32 ? float(at) : __half2float(at);
+        token_key = order_key(least, token);
+        if (single >= 0) before += order_key(value_at<F32>(row, single), single) > token_key;
+        // equal logits before the token in its own vector (the walk counts the larger ones there)
+        if (cta == 0 && tid >= 32 && tid < 32 + V::N && token_vec >= 0 && token_vec < nvec) {
+            const int i = head + token_vec * V::N + tid - 32;
+            if (i < token) before += value_at<F32>(row, i) == least;
+        }
+    };
     float step_max = -INFINITY;   // lane i: the warp's maximum in the steps i, i + 32, ..
-    auto take = [&](int start, int step) {
+
+    if (steps == 0) look_at_token();
+    for (int step = 0; step < steps; ++step) {
+        request(step + 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        V v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].set(ring[((step & 1) * U + u) * kThreads + tid]);
+        if (step + 1 == steps) {   // behind the end: adds nothing, and lies behind every token's vector
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (first + (step * U + u) * stride >= nvec) v[u].clear();
+        }
         float g = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u) g = v[u].max_with(g);
@@ -378,40 +415,34 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
         z_low += (z - (sum - part)) + (za - part);
         z = sum;
         t += ta + tb;
-        if (RANK && g >= least) {               // most tokens are likely ones: few vectors reach them
+        if (step == 0) look_at_token();
+        if (RANK && g >= least) {               // most tokens are likely ones: few steps reach them
             E thr[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) thr[u] = start + tid + u * kThreads < token_vec ? at : over;
+            for (int u = 0; u < U; ++u) thr[u] = first + (step * U + u) * stride < token_vec ? at : over;
             before += count_ge(v, thr);
-            if (token_key >> 32 == 0x007fffffu)   // a masked token: the vectors behind the end counted as equal
-                for (int u = 0; u < U; ++u) {
-                    const int i = start + tid + u * kThreads;
-                    if (i >= v1 && i < token_vec) before -= V::N;
-                }
         }
-    };
-    int step = 0;
-    for (int start = v0; start < v1; start += kStep, ++step) {
-        if (start + kStep < v1) fetch(next, start + kStep);
-        take(start, step);
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = next[u];
     }
 
     // ---- join: the warps leave their parts with the first CTA, and with every CTA what they reach
-    const Part own = joined(Part{m, m > -INFINITY ? (z - 1.f) + z_low : z, t}, p.scale2);
-    if (RANK) before = __reduce_add_sync(dq::kFull, before);
     const int warps = ctas * WARPS, me = cta * WARPS + warp;
-    // at least n groups of logits: whole warps, or if there are fewer, the k largest threads of each
+    const Part own = joined({Part{m, m > -INFINITY ? (z - 1.f) + z_low : z, t}}, p.scale2);
+    if (RANK) before = __reduce_add_sync(dq::kFull, before);
+    // one logit that a warp reaches, or with few warps its k largest threads: lane i the i-th
+    int k_shift = 0;
     float reach = own.m;
-    if (p.top_n > warps) {
-        const int k = (p.top_n + warps - 1) / warps;
-        float rest = m;
-        for (int i = 1; i < k; ++i) {
-            if (lane == __ffs(__ballot_sync(dq::kFull, rest == reach)) - 1) rest = -INFINITY;
-            reach = redux_max(rest);
+    if (p.top_n > 0 && warps < 32) {
+        k_shift = 1;
+        while (p.top_n > warps << k_shift) ++k_shift;
+        float rest = m, best = own.m;
+        for (int i = 1; i < 1 << k_shift; ++i) {
+            if (lane == __ffs(__ballot_sync(dq::kFull, rest == best)) - 1) rest = -INFINITY;
+            best = redux_max(rest);
+            if (lane == i) reach = best;
         }
     }
+    const int k_mask = (1 << k_shift) - 1;
+    reach = __shfl_sync(dq::kFull, reach, lane & k_mask);
     if (ctas > 1) cluster_wait();
     else __syncthreads();
     if (lane == 0) {
@@ -420,40 +451,47 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
         peer_store(peer_addr(&sh.t[me], 0), __float_as_uint(own.t));
         peer_store(peer_addr(&sh.before[me], 0), unsigned(before));
     }
-    if (p.top_n > 0 && lane < ctas) peer_store(peer_addr(&sh.reach[me], lane), __float_as_uint(reach));
+    if (p.top_n > 0 && lane >> k_shift < ctas) peer_store(peer_addr(&sh.reach[(me << k_shift) + (lane & k_mask)], lane >> k_shift), __float_as_uint(reach));
     sync_all();
 
     // ---- the candidates for the n best
     if (p.top_n > 0) {
-        int groups = 1;
-        while (groups < p.top_n) groups <<= 1;
-        // tau: the least of what the groups reach
-        float tau = -INFINITY;
-        for (int i = lane; i < warps; i += 32) tau = fmaxf(tau, sh.reach[i]);
-        if (warps < 32) tau = __shfl_sync(dq::kFull, tau, lane & (warps - 1));
-        if (p.top_n <= warps)
-            for (int off = groups; off < 32; off <<= 1) tau = fmaxf(tau, __shfl_xor_sync(dq::kFull, tau, off));
-        tau = redux_min(tau);
+        // up to 32 different logits that the row reaches, of 32 groups of warps or of the warps' largest threads; tau: the n-th of them
+        float x = -INFINITY;
+        if (warps >= 32)
+            for (int i = lane; i < warps; i += 32) x = fmaxf(x, sh.reach[i]);
+        else if (lane < warps << k_shift) x = sh.reach[lane];
+        sh.ranked[warp][lane] = x;
+        __syncwarp();
+        int place = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 o = reinterpret_cast<const float4*>(sh.ranked[warp])[i];
+            place += (o.x > x || (o.x == x && 4 * i < lane)) + (o.y > x || (o.y == x && 4 * i + 1 < lane)) + (o.z > x || (o.z == x && 4 * i + 2 < lane)) +
+                     (o.w > x || (o.w == x && 4 * i + 3 < lane));
+        }
+        const float tau = __shfl_sync(dq::kFull, x, __ffs(__ballot_sync(dq::kFull, place == p.top_n - 1)) - 1);
 
-        const uint32_t keys0 = peer_addr(sh.keys, 0), n0 = peer_addr(&sh.n_keys, 0);
+        const int room = kKeys / ctas;
+        const uint32_t keys0 = peer_addr(&sh.keys[cta * room], 0);
         auto flood = [&] { for (int i = 0; i < ctas; ++i) peer_store(peer_addr(&sh.flooded, i), 1u); };
         auto push = [&](float x, int i) {
-            const unsigned at_key = peer_add(n0, 1u);
-            if (at_key < unsigned(kKeys)) peer_store(keys0 + at_key * 8, order_key(x, i));
-            else flood();
+            const unsigned n = atomicAdd(&sh.n_own, 1u);
+            if (n < unsigned(room)) peer_store(keys0 + n * 8, order_key(x, i));
+            else if (n == unsigned(room)) flood();
         };
         if (tau > -INFINITY) {
             const unsigned has = __ballot_sync(dq::kFull, m >= tau);
             const int n_cand = __popc(has);
-            if (m >= tau) sh.cand[warp][__popc(has & ((1u << lane) - 1))] = tid;
+            if (m >= tau) sh.cand[warp][__popc(has & ((1u << lane) - 1))] = first;
             __syncwarp();
-            if (n_cand <= 16 || step <= 1) {
+            if (n_cand <= 16 || steps <= 1) {
                 // in the steps in which the warp reached tau, eight threads' four vectors at a time
-                for (unsigned steps = __ballot_sync(dq::kFull, step_max >= tau); steps; steps &= steps - 1)
-                    for (int j = __ffs(steps) - 1; j < step; j += 32)
+                for (unsigned in = __ballot_sync(dq::kFull, step_max >= tau); in; in &= in - 1)
+                    for (int step = __ffs(in) - 1; step < steps; step += 32)
                         for (int c = lane >> 2; c < n_cand; c += 8) {
-                            const int i = v0 + j * kStep + sh.cand[warp][c] + (lane & 3) * kThreads;
-                            if (i >= v1) continue;
+                            const int i = sh.cand[warp][c] + (step * U + (lane & 3)) * stride;
+                            if (i >= nvec) continue;
                             V w;
                             w.load(vecs + i);
                             if (w.max_with(-INFINITY) >= tau) {
@@ -463,22 +501,23 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
                             }
                         }
                 if (single >= 0) {
-                    const float x = value_at<F32>(row, single);
-                    if (x >= tau) push(x, single);
+                    const float y = value_at<F32>(row, single);
+                    if (y >= tau) push(y, single);
                 }
             } else if (lane == 0) flood();
             sync_all();
         }
         if (tau == -INFINITY || sh.flooded) {
-            // the whole part again, 32 sorted keys a warp
+            // the CTA's vectors again, 32 sorted keys a warp
             unsigned long long list = 0;
             offer_keys(list, single >= 0 ? order_key(value_at<F32>(row, single), single) : 0, p.top_n);
-            for (int base = v0 + warp * 32; base < v1; base += kThreads) {
+            for (int base = first - lane; base < nvec; base += stride) {
                 const int i = base + lane;
                 V w;
-                if (i < v1) w.load(vecs + i);
+                w.clear();
+                if (i < nvec) w.load(vecs + i);
 #pragma unroll
-                for (int e = 0; e < V::N; ++e) offer_keys(list, i < v1 && !(w.at(e) < tau) ? order_key(w.at(e), head + i * V::N + e) : 0, p.top_n);
+                for (int e = 0; e < V::N; ++e) offer_keys(list, i < nvec && !(w.at(e) < tau) ? order_key(w.at(e), head + i * V::N + e) : 0, p.top_n);
             }
             sh.lists[warp][lane] = list;
             for (int w = WARPS / 2; w >= 1; w >>= 1) {
@@ -488,49 +527,63 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
                     sh.lists[warp][lane] = list;
                 }
             }
-            if (warp == 0) {
-                if (lane < p.top_n) peer_store(keys0 + (cta * p.top_n + lane) * 8, list);
-                if (cta == 0 && lane == 0) sh.n_keys = ctas * p.top_n;
-            }
+            __syncthreads();
+            for (int i = tid; i < room; i += kThreads) peer_store(keys0 + i * 8, i < p.top_n ? sh.lists[0][i] : 0ull);
             sync_all();
         }
     }
     if (cta != 0) return;
 
-    // ---- the first CTA writes the row's answers
-    Part all{-INFINITY, 0.f, 0.f};
-    for (int i = lane; i < warps; i += 32) all = joined(all, Part{sh.m[i], sh.z[i], sh.t[i]}, p.scale2);
-    all = joined(all, p.scale2);
-    const bool none = all.m == -INFINITY && all.z == 0.f;   // masked altogether
-    const float lnz = log1pf(all.z);
-    // the difference is taken before the scale: a row of the type's lowest value would overflow the product
-    auto logprob_of = [&](float x) { return none ? -INFINITY : (x - all.m) * p.inv_temp - lnz; };
-    if (warp == 0) {
+    // ---- the first CTA writes the row's answers: its last warp joins the parts, and all of them order the keys
+    if (warp == WARPS - 1) {
+        constexpr int N = kMaxCluster * WARPS / 32;
+        Part parts[N];
         int rank = 0;
-        if (RANK) {
-            for (int i = lane; i < warps; i += 32) rank += sh.before[i];
-            rank = __reduce_add_sync(dq::kFull, rank);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int w = lane + 32 * i;
+            parts[i] = w < warps ? Part{sh.m[w], sh.z[w], sh.t[w]} : Part{-INFINITY, 0.f, 0.f};
+            if (RANK && w < warps) rank += sh.before[w];
         }
+        const Part all = joined(parts, p.scale2);
+        if (RANK) rank = __reduce_add_sync(dq::kFull, rank);
+        const bool none = all.m == -INFINITY && all.z == 0.f;   // masked altogether
+        const float lnz = log1pf(all.z);
         if (lane == 0) {
-            if (RANK && p.logprob) p.logprob[r] = real ? logprob_of(key_value(token_key)) : 0.f;
+            sh.row_m = all.m;
+            sh.row_lnz = lnz;
+            sh.none = none;
+            if (p.entropy) p.entropy[r] = none ? 0.f : lnz - __fdividef(all.t, 1.f + all.z) * kLn2;
+            // the difference is taken before the scale: a row of the type's lowest value would overflow the product
+            if (RANK && p.logprob) p.logprob[r] = !real ? 0.f : none ? -INFINITY : (least - all.m) * p.inv_temp - lnz;
             if (RANK && p.rank) p.rank[r] = real && token_key >> 32 ? rank : -1;
-            if (p.entropy) p.entropy[r] = none ? 0.f : lnz - all.t / (1.f + all.z) * kLn2;
         }
     }
-    if (p.top_n > 0) {   // four threads count the keys before one
-        const int n_keys = int(sh.n_keys), part = tid & 3;
-        for (int base = 0; base < n_keys; base += kThreads / 4) {
-            const int k = base + (tid >> 2);
-            const unsigned long long key = k < n_keys ? sh.keys[k] : 0;
-            int place = 0;
+    if (p.top_n == 0) return;
+    unsigned long long* list = &sh.lists[0][0];
+    for (int i = tid; i < kKeys; i += kThreads) {
+        const unsigned long long key = sh.keys[i];
+        const unsigned has = __ballot_sync(dq::kFull, key != 0);
+        if (has) {
+            unsigned base = 0;
+            if (lane == 0) base = atomicAdd(&sh.n_keys, __popc(has));
+            base = __shfl_sync(dq::kFull, base, 0) + __popc(has & ((1u << lane) - 1));
+            if (key != 0) list[base] = key;
+        }
+    }
+    __syncthreads();
+    const int n_keys = int(sh.n_keys), quarter = tid & 3;
+    for (int base = 0; base < n_keys; base += kThreads / 4) {   // four threads count the keys before one
+        const int k = base + (tid >> 2);
+        const unsigned long long key = k < n_keys ? list[k] : 0;
+        int place = 0;
 #pragma unroll 4
-            for (int i = part; i < n_keys; i += 4) place += sh.keys[i] > key;
-            place += __shfl_xor_sync(dq::kFull, place, 1);
-            place += __shfl_xor_sync(dq::kFull, place, 2);
-            if (part == 0 && key != 0 && place < p.top_n) {
-                p.top_idx[r * p.top_n + place] = int(0xffffffffu - unsigned(key));
-                p.top_logprob[r * p.top_n + place] = logprob_of(key_value(key));
-            }
+        for (int i = quarter; i < n_keys; i += 4) place += list[i] > key;
+        place += __shfl_xor_sync(dq::kFull, place, 1);
+        place += __shfl_xor_sync(dq::kFull, place, 2);
+        if (quarter == 0 && key != 0 && place < p.top_n) {
+            p.top_idx[r * p.top_n + place] = int(0xffffffffu - unsigned(key));
+            p.top_logprob[r * p.top_n + place] = sh.none ? -INFINITY : (key_value(key) - sh.row_m) * p.inv_temp - sh.row_lnz;
         }
     }
 }
@@ -543,11 +596,13 @@ void launch(const LogprobParams& p, int ctas, cudaStream_t st)
     const int dev = current_device();
     if (!set[dev]) {
         cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "logprobs cluster attribute");
+        cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * kRingBytes), "logprobs smem attribute");
         set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(p.rows) * unsigned(ctas));
     cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = WARPS * kRingBytes;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
