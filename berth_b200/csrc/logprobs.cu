@@ -622,12 +622,24 @@ void launch(const LogprobParams& p, int ctas, int warps, cudaStream_t st)
     else launch<F32, RANK, 16>(p, ctas, st);
 }
 
-// CTAs a row is split over and warps of each.
+// How a row is split: CTAs of its cluster and warps of each.  Measured (us, rows x vocabulary, warps/CTAs):
+//   as many warps as run at once (4736), a power of two of them a row, none with less than 1 KB:
+//     32 x 248320 fp32 128 warps 13.6, 64 warps 16.2; 64 x 248320 fp16 64 warps 15.1, 128 warps 21.2; 1 x 5000 fp32 16 warps 4.8, 64 warps 5.0;
+//     at most 128: 16 x 248320 fp32 12.2, 256 warps 14.6;
+//   a second wave where the first would leave a quarter of the GPU idle and the parts are long:
+//     421 x 248320 fp16 16 warps 50.7, 8 warps 63.2; 150 x 250000 fp16 32 warps 27.1, 16 warps 34.9; not for 77 x 100003 fp32 (13.2 both);
+//   large clusters of small CTAs for few rows (1 x 32000 fp16 4/8 5.1, 16/2 6.2; 4 x 248320 fp32 8/16 7.6, 16/8 8.7), at most 8 CTAs
+//     above 16 rows (32 x 248320 fp32 16/8 13.6, 8/16 16.5), single CTAs above 148 rows of up to 16 warps (421 rows 16/1 50.7, 4/4 55.1).
 void row_split(int rows, long long row_bytes, int& ctas, int& warps)
 {
-    warps = row_bytes <= 16384 ? 4 : 16;
-    ctas = 1;
-    while (ctas < 16 && rows * ctas * 2 <= 296 && row_bytes / ctas > 32768) ctas *= 2;
+    const long long at_once = 148 * 32;
+    long long n = 4;
+    while (n < 128 && rows * n * 2 <= at_once && row_bytes >= n * 2 * 1024) n *= 2;
+    if (n < 128 && 4 * rows * n <= 3 * at_once && row_bytes > n * 16384) n *= 2;
+    if (n < 128 && rows > 148 && row_bytes > n * 49152) n *= 2;
+    const long long most = rows <= 16 ? 16 : rows <= 148 || n > 16 ? 8 : 1;
+    warps = int(std::min<long long>(16, std::max<long long>(4, n / most)));
+    ctas = int(n / warps);
 }
 
 }  // namespace
