@@ -14,6 +14,7 @@ struct RopeParams {
     const int32_t* positions;
     const double* inv_freq;
     int tokens, dim, rot, half_rot, interleaved;
+    int lanes, tile;   // lanes of a head (a power of two), tokens of a block (a power of two)
     float factor, eps, bias;
 };
 
@@ -38,41 +39,248 @@ __device__ __forceinline__ float2 turn(int position, double inv_freq, float fact
     return make_float2(c * factor, s * factor);
 }
 
-// One warp per (token, head); a lane reads and writes both elements of its pairs, so y may be x.
-template <typename T>
-__global__ void __launch_bounds__(128) k_rope(const RopeParams p)
+// Sixteen elements of a head, as two pieces of eight (kHalf: i.. and i + rot / 2.. , so that a lane holds both elements of its
+// eight pairs), in 16-byte accesses.
+template <typename T> struct Piece;
+template <> struct Piece<__half> {
+    uint4 v;
+    __device__ __forceinline__ void load(const __half* p) { v = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void get(float* x) const
+    {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ void store(__half* p, const float* x)
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <> struct Piece<float> {
+    float4 v[2];
+    __device__ __forceinline__ void load(const float* p) { v[0] = reinterpret_cast<const float4*>(p)[0]; v[1] = reinterpret_cast<const float4*>(p)[1]; }
+    __device__ __forceinline__ void get(float* x) const
+    {
+        x[0] = v[0].x; x[1] = v[0].y; x[2] = v[0].z; x[3] = v[0].w; x[4] = v[1].x; x[5] = v[1].y; x[6] = v[1].z; x[7] = v[1].w;
+    }
+    static __device__ __forceinline__ void store(float* p, const float* x)
+    {
+        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+};
+__device__ __forceinline__ void norm8(float* x, const void* w, int at, float rinv, float bias)
 {
+    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + at);
+    const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = x[2 * i] * rinv * (__uint_as_float(h[i] << 16) + bias);
+        x[2 * i + 1] = x[2 * i + 1] * rinv * (__uint_as_float(h[i] & 0xffff0000u) + bias);
+    }
+}
+
+constexpr int kThreads = 256, kTable = 2048;   // cos / sin pairs a block holds
+
+// A block takes p.tile tokens: it fills a table of their cos and sin (one thread per pair and token, 64-bit angles), then groups of
+// p.lanes lanes walk the heads, each lane sixteen elements of a head.  A group stays with its token, so a lane's eight pairs of cos
+// and sin stay in registers.  kHalf / kNeighbours: wide accesses, rotated pieces of whole eights.
+enum { kHalf = 0, kNeighbours = 1 };
+template <typename T, int MODE, bool NORM>
+__global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
+{
+    __shared__ __align__(16) float2 table[kTable];
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31, heads = p.r[0].heads + p.r[1].heads;
-    const long long total = (long long) p.tokens * heads;
-    for (long long item = (long long) blockIdx.x * 4 + (threadIdx.x >> 5); item < total; item += (long long) gridDim.x * 4) {
-        const int t = int(item / heads), hh = int(item % heads);
-        const berth_rope_rows& r = p.r[hh >= p.r[0].heads];
-        const int h = hh >= p.r[0].heads ? hh - p.r[0].heads : hh;
-        const T* x = static_cast<const T*>(r.x) + t * r.x_token + h * r.x_head;
-        T* y = static_cast<T*>(r.y) + t * r.y_token + h * r.y_head;
-        float rinv = 1.f;
-        if (r.norm) {
-            float s = 0.f;
-            for (int i = lane; i < p.dim; i += 32) { const float v = to_f(x[i]); s = fmaf(v, v, s); }
+    const int tid = threadIdx.x, heads = p.r[0].heads + p.r[1].heads;
+    const int group = tid / p.lanes, lane = tid % p.lanes, groups_per_token = kThreads / p.lanes / p.tile;
+    const int slot = group / groups_per_token, t0 = blockIdx.x * p.tile, t = t0 + slot;
+    // the lane's pieces: offsets of eight elements, -1 = none
+    const int turning = MODE == kHalf ? p.half_rot / 8 : (p.rot + 15) / 16;   // lanes that turn something
+    int at[2];
+    if (lane < turning) {
+        at[0] = MODE == kHalf ? 8 * lane : 16 * lane;
+        at[1] = at[0] + (MODE == kHalf ? p.half_rot : 8);
+    } else {
+        at[0] = (MODE == kHalf ? p.rot : 16 * turning) + 16 * (lane - turning);
+        at[1] = at[0] + 8;
+    }
+    if (at[0] >= p.dim) at[0] = -1;
+    if (at[1] >= p.dim) at[1] = -1;
+
+    auto rows_of = [&](int h, const T*& x, T*& y, const void*& norm) {
+        const berth_rope_rows& r = p.r[h >= p.r[0].heads];
+        const long long hh = h >= p.r[0].heads ? h - p.r[0].heads : h;
+        x = static_cast<const T*>(r.x) + t * r.x_token + hh * r.x_head;
+        y = static_cast<T*>(r.y) + t * r.y_token + hh * r.y_head;
+        norm = r.norm;
+    };
+    const int step = groups_per_token * gridDim.y;
+    int h = blockIdx.y * groups_per_token + group % groups_per_token;
+    Piece<T> in[2];
+    const T* x = nullptr;
+    T* y = nullptr;
+    const void* norm = nullptr;
+    auto fetch = [&] {
+        if (t < p.tokens && h < heads) {
+            rows_of(h, x, y, norm);
 #pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(dq::kFull, s, off);
-            rinv = 1.0f / sqrtf(s / float(p.dim) + p.eps);
+            for (int i = 0; i < 2; ++i)
+                if (at[i] >= 0) in[i].load(x + at[i]);
         }
-        auto in = [&](int i) {
-            const float v = to_f(x[i]);
-            return r.norm ? v * rinv * (bf16_at(r.norm, i) + p.bias) : v;
-        };
-        const int pos = p.positions[t];
-        for (int i = lane; i < p.half_rot; i += 32) {
-            const float2 cs = turn(pos, p.inv_freq[i], p.factor);
-            const int a = p.interleaved ? 2 * i : i, b = p.interleaved ? 2 * i + 1 : i + p.half_rot;
-            const float xa = in(a), xb = in(b);
-            y[a] = from_f<T>(xa * cs.x - xb * cs.y);
-            y[b] = from_f<T>(xb * cs.x + xa * cs.y);
+    };
+    fetch();
+    for (int i = tid; i < p.tile * p.half_rot; i += kThreads) {
+        const int s = i / p.half_rot;
+        if (t0 + s < p.tokens) table[i] = turn(p.positions[t0 + s], p.inv_freq[i - s * p.half_rot], p.factor);
+    }
+    __syncthreads();
+    float2 cs[8];
+    if (lane < turning) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (8 * lane + i < p.half_rot) cs[i] = table[slot * p.half_rot + 8 * lane + i];
+    }
+    // every lane of a warp walks alike, so that the norm's sums meet
+    for (int round = h; round - group % groups_per_token < heads; round += step) {
+        float v[16];
+        T* to = y;
+        const void* w = norm;
+        const bool live = t < p.tokens && h < heads;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (live && at[i] >= 0) in[i].get(v + 8 * i);
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[8 * i + j] = 0.f;
+            }
+        h += step;
+        fetch();
+        if constexpr (NORM) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s = fmaf(v[j], v[j], s);
+            for (int off = p.lanes / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(dq::kFull, s, off);
+            if (live && w) {
+                const float rinv = rsqrtf(s / float(p.dim) + p.eps);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (at[i] >= 0) norm8(v + 8 * i, w, at[i], rinv, p.bias);
+            }
         }
-        for (int i = p.rot + lane; i < p.dim; i += 32) y[i] = from_f<T>(in(i));
+        if (lane < turning) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (MODE == kNeighbours && 8 * lane + i >= p.half_rot) break;   // the rest of the last lane is passed on
+                float &a = MODE == kHalf ? v[i] : v[2 * i], &b = MODE == kHalf ? v[8 + i] : v[2 * i + 1];
+                const float a0 = a, b0 = b;
+                a = a0 * cs[i].x - b0 * cs[i].y;
+                b = b0 * cs[i].x + a0 * cs[i].y;
+            }
+        }
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (at[i] >= 0) Piece<T>::store(to + at[i], v + 8 * i);
+        }
+    }
+}
+
+// The same for any part, alignment and stride: a lane holds sixteen consecutive elements and finds the other element of a pair
+// in shared memory (pitch 17, so that lanes 16 elements apart meet different banks).
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(kThreads) k_rope_any(const RopeParams p, bool wide)
+{
+    __shared__ float2 table[kTable + kTable / 16 + kThreads];   // (pitch: half_rot + half_rot / 16 + 1, at most kThreads tokens)
+    __shared__ float stage[kThreads * 17];
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x, heads = p.r[0].heads + p.r[1].heads;
+    const int group = tid / p.lanes, lane = tid % p.lanes, groups_per_token = kThreads / p.lanes / p.tile;
+    const int slot = group / groups_per_token, t0 = blockIdx.x * p.tile, t = t0 + slot, e0 = 16 * lane;
+    const int pitch = p.half_rot + p.half_rot / 16 + 1;
+    for (int i = tid; i < p.tile * p.half_rot; i += kThreads) {
+        const int s = i / p.half_rot, k = i - s * p.half_rot;
+        if (t0 + s < p.tokens) table[s * pitch + k + k / 16] = turn(p.positions[t0 + s], p.inv_freq[k], p.factor);
+    }
+    __syncthreads();
+    float* mine = stage + (tid - lane) * 17;   // the group's head
+    const float2* cs = table + slot * pitch;
+    const int step = groups_per_token * gridDim.y, h0 = blockIdx.y * groups_per_token;
+    for (int base = h0; base < heads; base += step) {
+        const int h = base + group % groups_per_token;
+        const bool live = t < p.tokens && h < heads;
+        const berth_rope_rows& r = p.r[h >= p.r[0].heads];
+        const long long hh = h >= p.r[0].heads ? h - p.r[0].heads : h;
+        const T* x = static_cast<const T*>(r.x) + t * r.x_token + hh * r.x_head;
+        T* y = static_cast<T*>(r.y) + t * r.y_token + hh * r.y_head;
+        float v[16];
+        if (wide && live && e0 + 16 <= p.dim) {
+            Piece<T> a, b;
+            a.load(x + e0);
+            b.load(x + e0 + 8);
+            a.get(v);
+            b.get(v + 8);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = live && e0 + j < p.dim ? to_f(x[e0 + j]) : 0.f;
+        }
+        if constexpr (NORM) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s = fmaf(v[j], v[j], s);
+            for (int off = p.lanes / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(dq::kFull, s, off);
+            if (live && r.norm) {
+                const float rinv = rsqrtf(s / float(p.dim) + p.eps);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (e0 + j < p.dim) v[j] = v[j] * rinv * (bf16_at(r.norm, e0 + j) + p.bias);
+            }
+        }
+        if (p.interleaved) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 2)
+                if (e0 + j < p.rot) {
+                    const int k = (e0 + j) / 2;
+                    const float2 c = cs[k + k / 16];
+                    const float a = v[j], b = v[j + 1];
+                    v[j] = a * c.x - b * c.y;
+                    v[j + 1] = b * c.x + a * c.y;
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mine[lane * 17 + j] = v[j];
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int e = e0 + j;
+                if (e < p.rot) {
+                    const bool second = e >= p.half_rot;
+                    const int k = second ? e - p.half_rot : e, o = second ? k : e + p.half_rot;
+                    const float2 c = cs[k + k / 16];
+                    const float other = mine[o + o / 16];
+                    v[j] = second ? v[j] * c.x + other * c.y : v[j] * c.x - other * c.y;
+                }
+            }
+            __syncwarp();
+        }
+        if (!live) continue;
+        if (wide && e0 + 16 <= p.dim) {
+            Piece<T>::store(y + e0, v);
+            Piece<T>::store(y + e0 + 8, v + 8);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (e0 + j < p.dim) y[e0 + j] = from_f<T>(v[j]);
+        }
     }
 }
 
@@ -88,6 +296,58 @@ berth_rope_rows checked_rows(const berth_rope_rows& r, const char* what, int tok
     if ((tokens > 1 && std::llabs(c.y_token) < dim) || (c.heads > 1 && std::llabs(c.y_head) < dim)) fail("the heads of the output overlap");
     if (c.x == c.y && (c.x_token != c.y_token || c.x_head != c.y_head)) fail("an output in place needs the strides of its input");
     return c;
+}
+
+// Every row of 16-byte pieces: pointers and strides.
+bool wide_rows(const RopeParams& p, int size)
+{
+    for (const berth_rope_rows& r : p.r) {
+        if (r.heads == 0) continue;
+        const uintptr_t bits = reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.y) | reinterpret_cast<uintptr_t>(r.norm) |
+                               uintptr_t(r.x_token * size) | uintptr_t(r.x_head * size) | uintptr_t(r.y_token * size) | uintptr_t(r.y_head * size);
+        if (bits & 15) return false;
+    }
+    return true;
+}
+
+std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
+{
+    const int heads = p.r[0].heads + p.r[1].heads;
+    const bool wide = wide_rows(p, f32 ? 4 : 2) && p.dim % 8 == 0, norm = p.r[0].norm || p.r[1].norm;
+    const bool eights = wide && (p.interleaved ? p.rot % 8 == 0 : p.half_rot % 8 == 0);
+    // lanes: pieces that turn, then what is passed on
+    int units = (p.dim + 15) / 16;
+    if (eights) {
+        const int turning = p.interleaved ? (p.rot + 15) / 16 : p.half_rot / 8, passed = p.interleaved ? 16 * turning : p.rot;
+        units = turning + std::max(0, (p.dim - passed + 15) / 16);
+    }
+    p.lanes = 1;
+    while (p.lanes < units) p.lanes *= 2;
+    const int groups = kThreads / p.lanes;
+    // tokens of a block: until every group walks some four heads, as long as the grid has four blocks an SM
+    p.tile = 1;
+    while (p.tile < groups && heads * p.tile < 4 * groups && (p.tokens + 2 * p.tile - 1) / (2 * p.tile) >= 148 * 4 && 2 * p.tile * p.half_rot <= kTable)
+        p.tile *= 2;
+    // few tokens: their heads over several blocks
+    const int blocks_x = (p.tokens + p.tile - 1) / p.tile;
+    int blocks_y = 1;
+    while (blocks_x * blocks_y < 148 && blocks_y * groups / p.tile < heads) ++blocks_y;
+    const dim3 grid(blocks_x, blocks_y);
+    std::string name;
+    auto go = [&](auto kern, const char* what, auto... more) {
+        launch_pdl(kern, grid, dim3(kThreads), 0, st, "rope launch", p, more...);
+        name = std::string(what) + "<" + (f32 ? "float" : "half") + (norm ? ",norm" : "") + ">";
+    };
+    auto typed = [&](auto zero) {
+        using T = decltype(zero);
+        if (!eights) norm ? go(k_rope_any<T, true>, "k_rope_any", wide) : go(k_rope_any<T, false>, "k_rope_any", wide);
+        else if (p.interleaved) norm ? go(k_rope<T, kNeighbours, true>, "k_rope_neighbours") : go(k_rope<T, kNeighbours, false>, "k_rope_neighbours");
+        else norm ? go(k_rope<T, kHalf, true>, "k_rope_half") : go(k_rope<T, kHalf, false>, "k_rope_half");
+    };
+    if (f32) typed(0.0f);
+    else typed(__half{});
+    return name + " block=" + std::to_string(kThreads) + " grid=" + std::to_string(blocks_x) + "x" + std::to_string(blocks_y) + " tokens=" +
+           std::to_string(p.tile) + " lanes=" + std::to_string(p.lanes);
 }
 
 }  // namespace
@@ -114,10 +374,7 @@ extern "C" int berth_ops_rope(const berth_rope_rows* q, const berth_rope_rows* k
         if (k) p.r[1] = checked_rows(*k, "k", n_tokens, head_dim);
         p.positions = positions; p.inv_freq = inv_freq; p.tokens = n_tokens; p.dim = head_dim; p.rot = rot_dim; p.half_rot = rot_dim / 2;
         p.interleaved = interleaved != 0; p.factor = attention_factor; p.eps = norm_epsilon; p.bias = norm_bias;
-        const long long items = (long long) n_tokens * (p.r[0].heads + p.r[1].heads);
-        const int grid = int(std::min<long long>((items + 3) / 4, 148LL * 16));
-        launch_pdl(fp32 ? k_rope<float> : k_rope<__half>, dim3(grid), dim3(128), 0, (cudaStream_t) stream, "rope launch", p);
-        st.launch = std::string("k_rope<") + (fp32 ? "float" : "half") + "> block=128 grid=" + std::to_string(grid);
+        st.launch = launch_rope(p, fp32 != 0, (cudaStream_t) stream);
     });
 }
 
