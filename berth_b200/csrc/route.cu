@@ -3,6 +3,7 @@
 #include "exl3_decode.cuh"
 #include "route.cuh"
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 
@@ -53,12 +54,6 @@ __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(dq::kFull, v, off);
-    return v;
-}
-__device__ __forceinline__ float warp_max(float v)   // NaN is ignored
-{
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(dq::kFull, v, off));
     return v;
 }
 
@@ -149,63 +144,219 @@ __device__ __noinline__ int choose64(const float (&l)[PER], int cnt, int base, i
     return mine;
 }
 
+__device__ __forceinline__ float redux_max(float v) { float r; asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float redux_min(float v) { float r; asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
 // One warp per token; lane = P lanes per group, q consecutive experts each.
+//
+// The choice is made in 32 bits first and in 64 only where that cannot tell: an expert's key is the order of its fp32 choice
+// score with the lowest log2(PER) bits replaced by its place in the lane, a lane keeps its keys sorted, and a round takes the
+// largest head of the 32 lanes (one redux, one ballot).  Where two neighbours in the order, the first expert not chosen among them,
+// or the last group kept and the first one dropped, lie closer than both scores' errors, the warp repeats the choice in 64 bits.
+// Errors of c = s + b in units of 2^-24: sigmoid, s (1 - s) (1.5 |l| + 4) for exp and 3 for sum and reciprocal, below 4.5 each;
+// softmax, s (2.5 |l - m| + 7) <= 9 each and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below 2 (28 + PER) for a pair; the sum
+// with the bias |c|; the place bits 2 PER |c|.  fp16 logits ordered by themselves lose nothing to the place bits: never repeated.
 template <int PER, bool F32, int SCORE>   // SCORE: kSigmoid or kSoftmax
-__global__ void __launch_bounds__(128) k_moe_route(const RouteParams p, bool by_logit, bool top2)
+__global__ void __launch_bounds__(128) k_moe_route(const RouteParams p, bool by_logit, bool top2, bool wide)
 {
+    constexpr unsigned kMask = PER - 1;
+    constexpr bool kSorted = PER <= 8;
+    constexpr float kLog2e = 1.44269504088896341f, kUnit = 1.f / (1 << 24);
+    __shared__ uint2 chosen[4][33];
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31, t = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (t >= p.T) return;
-    const char* row = static_cast<const char*>(p.logits) + size_t(t) * p.ld * (F32 ? 4 : 2);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane / p.P, first = (lane % p.P) * p.q;
     const int cnt = g < p.G ? min(max(p.gs - first, 0), p.q) : 0;
     const int base = g < p.G ? g * p.gs + first : 0;
-    float l[PER];
-    bool nan = false;
+    const float tol = by_logit ? (F32 ? 0.f : -1.f) : kUnit * (SCORE == kSigmoid ? 9.f : 2.f * (28 + PER));
+    const float tol_rel = by_logit ? 0.f : kUnit * (2.f + 2.f * PER);
+    auto fetch = [&](int t, float (&l)[PER]) {
+        const char* row = static_cast<const char*>(p.logits) + size_t(t) * p.ld * (F32 ? 4 : 2);
+        if (PER >= 4 && wide) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        l[i] = i < cnt ? logit_at<F32>(row, base + i) : -INFINITY;
-        nan |= l[i] != l[i];
-    }
-    nan = __any_sync(dq::kFull, nan);
-    const int mine = choose64<PER>(l, cnt, base, by_logit ? kByLogit : SCORE, top2, p);
+            for (int i = 0; i < PER; i += 4) {
+                float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (i < cnt) {
+                    if constexpr (F32) {
+                        const float4 w = *reinterpret_cast<const float4*>(row + size_t(base + i) * 4);
+                        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(row + size_t(base + i) * 2);
+                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+                        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) l[PER >= 4 ? i + j : 0] = v[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) l[i] = i < cnt ? (F32 ? reinterpret_cast<const float*>(row)[base + i] : __half2float(reinterpret_cast<const __half*>(row)[base + i])) : -INFINITY;
+        }
+    };
+    const int stride = gridDim.x * 4;
+    float next[PER];
+    int t = blockIdx.x * 4 + warp;
+    if (t < p.T) fetch(t, next);
+    for (; t < p.T; t += stride) {
+        const char* row = static_cast<const char*>(p.logits) + size_t(t) * p.ld * (F32 ? 4 : 2);
+        float l[PER];
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            l[i] = clamp_logit(next[i]);
+            nan |= l[i] != l[i];
+        }
+        if (t + stride < p.T) fetch(t + stride, next);
 
-    // the weight of this lane's expert, fp32
-    const float v = lane < p.k ? logit_at<F32>(row, mine) : -INFINITY;
-    float w;
-    if (p.renorm) {
-        const float m = warp_max(v);
-        // relative to the largest of the chosen; a sigmoid far below zero is exp of its logit (within 2^-43)
-        if (SCORE == kSoftmax || m < -30.f) w = v > -INFINITY ? expf(v - m) : 0.f;
-        else w = 1.f / (1.f + expf(-v));
-        if (lane >= p.k) w = 0.f;
-        const float sum = warp_sum(w);
-        w = sum > 0.f ? w / sum : 0.f;
-    } else if (SCORE == kSigmoid) {
-        w = 1.f / (1.f + expf(-v));
-    } else {
-        float m = -INFINITY, z = 0.f;
+        // ---- choice scores in fp32
+        float m = -INFINITY, z = 0.f;   // softmax over all experts
+        const bool whole = SCORE == kSoftmax && (!by_logit || !p.renorm);
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) m = fmaxf(m, l[i]);
-        m = warp_max(m);
+            for (int i = 0; i < PER; ++i) m = fmaxf(m, l[i]);
+            m = redux_max(m);
+        }
+        float c[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (l[i] > -INFINITY) z += expf(l[i] - m);
-        z = warp_sum(z);
-        w = v > -INFINITY ? expf(v - m) / z : 0.f;
-    }
-    if (lane < p.k) {
-        p.idx[size_t(t) * p.k + lane] = mine;
-        p.w[size_t(t) * p.k + lane] = nan ? NAN : w * p.scale;
+        for (int i = 0; i < PER; ++i) {
+            c[i] = l[i];
+            if (SCORE == kSigmoid) {
+                if (!by_logit && l[i] > -INFINITY) c[i] = rcp(1.f + ex2(-l[i] * kLog2e));
+            } else if (whole) {
+                const float e = l[i] > -INFINITY ? ex2((l[i] - m) * kLog2e) : 0.f;
+                z += e;
+                if (!by_logit && l[i] > -INFINITY) c[i] = e;
+            }
+        }
+        if (whole) z = warp_sum(z);
+        if (!by_logit) {
+            const float inv = SCORE == kSoftmax ? rcp(z) : 1.f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (i < cnt && l[i] > -INFINITY) {
+                    if (SCORE == kSoftmax) c[i] *= inv;
+                    if (p.bias) c[i] += p.bias[base + i];
+                }
+        }
+
+        // ---- groups
+        bool unsure = false, dropped = false;
+        if (p.keep < p.G) {
+            float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                b2 = fmaxf(b2, fminf(b1, c[i]));   // (NaN: neither changes; a padded place is -inf)
+                b1 = fmaxf(b1, c[i]);
+            }
+            for (int off = 1; off < p.P; off <<= 1) {
+                const float o1 = __shfl_xor_sync(dq::kFull, b1, off), o2 = __shfl_xor_sync(dq::kFull, b2, off);
+                b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+                b1 = fmaxf(b1, o1);
+            }
+            const float score = top2 && b2 > -INFINITY ? b1 + b2 : b1;
+            int before = 0;
+            for (int j = 0; j < p.G; ++j) {
+                const float o = __shfl_sync(dq::kFull, score, j * p.P);
+                before += o > score || (o == score && j < g);
+            }
+            dropped = before >= p.keep;
+            const float least = redux_min(g < p.G && !dropped ? score : INFINITY), most = redux_max(g < p.G && dropped ? score : -INFINITY);
+            const float size = redux_max(b1 > -INFINITY ? fabsf(b1) + (b2 > -INFINITY ? fabsf(b2) : 0.f) : 0.f);   // what the sums' roundings scale with
+            unsure = least - most <= (by_logit ? -1.f : 2.f * tol + tol_rel * size);
+        }
+
+        // ---- keys, largest first
+        unsigned key[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const unsigned b = __float_as_uint(c[i] + 0.f);
+            const unsigned o = c[i] != c[i] ? 0x80u : ((b >> 31) ? ~b : b | 0x80000000u);
+            key[i] = i < cnt && !dropped ? (o & ~kMask) | (kMask - i) : 0u;
+        }
+        if constexpr (kSorted && PER > 1) {
+#pragma unroll
+            for (int span = 2; span <= PER; span *= 2)      // bitonic, descending
+#pragma unroll
+                for (int d = span / 2; d >= 1; d /= 2)
+#pragma unroll
+                    for (int i = 0; i < PER; ++i)
+                        if (!(i & d)) {
+                            const int j = d == span / 2 ? (i | (span - 1)) - (i & (span / 2 - 1)) : i + d;   // first step of a span: mirrored
+                            const unsigned hi = max(key[i], key[j]), lo = min(key[i], key[j]);
+                            key[i] = hi;
+                            key[j] = lo;
+                        }
+        }
+        unsigned head = key[0];
+        if constexpr (!kSorted) {
+#pragma unroll
+            for (int i = 1; i < PER; ++i) head = max(head, key[i]);
+        }
+        for (int s = 0; s <= p.k; ++s) {     // one more than is chosen: the first that is not
+            const unsigned top = __reduce_max_sync(dq::kFull, head & ~kMask);
+            const int owner = __ffs(__ballot_sync(dq::kFull, (head & ~kMask) == top)) - 1;
+            if (lane == owner) {
+                chosen[warp][s] = make_uint2(unsigned(base) + (kMask - (head & kMask)), top);
+                if constexpr (kSorted) {
+#pragma unroll
+                    for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1];
+                    key[PER - 1] = 0;
+                    head = key[0];
+                } else {
+                    unsigned h = 0;
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) {
+                        key[i] = key[i] == head ? 0u : key[i];
+                        h = max(h, key[i]);
+                    }
+                    head = h;
+                }
+            }
+        }
+        __syncwarp();
+        int mine = 0;
+        if (lane < p.k) {
+            const uint2 a = chosen[warp][lane], b = chosen[warp][lane + 1];
+            auto value = [](unsigned o) { return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o); };   // below -FLT_MAX: NaN, which is never unsure
+            const float va = value(a.y), vb = value(b.y);
+            mine = int(a.x);
+            unsure |= b.y != 0u && va - vb <= tol + tol_rel * fmaxf(fabsf(va), fabsf(vb));
+        }
+        __syncwarp();
+        if (__any_sync(dq::kFull, unsure)) mine = choose64<PER>(l, cnt, base, by_logit ? kByLogit : SCORE, top2, p);
+        nan = __any_sync(dq::kFull, nan);
+
+        // ---- the weight of this lane's expert
+        const float v = lane < p.k ? logit_at<F32>(row, mine) : -INFINITY;
+        float w;
+        if (p.renorm) {
+            const float most = redux_max(v);
+            // relative to the largest of the chosen; a sigmoid far below zero is exp of its logit (within 2^-43)
+            if (SCORE == kSoftmax || most < -30.f) w = v > -INFINITY ? expf(v - most) : 0.f;
+            else w = 1.f / (1.f + expf(-v));
+            if (lane >= p.k) w = 0.f;
+            const float sum = warp_sum(w);
+            w = sum > 0.f ? w / sum : 0.f;
+        } else if (SCORE == kSigmoid) {
+            w = 1.f / (1.f + expf(-v));
+        } else {
+            w = v > -INFINITY ? expf(v - m) / z : 0.f;
+        }
+        if (lane < p.k) {
+            p.idx[size_t(t) * p.k + lane] = mine;
+            p.w[size_t(t) * p.k + lane] = nan ? NAN : w * p.scale;
+        }
     }
 }
 
 template <int PER>
-void launch(bool f32, int score, const RouteParams& p, bool by_logit, bool top2, cudaStream_t st)
+void launch(bool f32, int score, const RouteParams& p, bool by_logit, bool top2, bool wide, int blocks, cudaStream_t st)
 {
-    const dim3 grid((p.T + 3) / 4), block(128);
-    auto go = [&](auto kern) { launch_pdl(kern, grid, block, 0, st, "k_moe_route launch", p, by_logit, top2); };
+    auto go = [&](auto kern) { launch_pdl(kern, dim3(blocks), dim3(128), 0, st, "k_moe_route launch", p, by_logit, top2, wide); };
     if (f32) score == kSigmoid ? go(k_moe_route<PER, true, kSigmoid>) : go(k_moe_route<PER, true, kSoftmax>);
     else score == kSigmoid ? go(k_moe_route<PER, false, kSigmoid>) : go(k_moe_route<PER, false, kSoftmax>);
 }
@@ -244,17 +395,22 @@ std::string route_tokens(const void* logits, bool f32, long long ld, const berth
     const int score = r.score == 1 ? kSigmoid : kSoftmax;
     int per = 1;
     while (per < p.q) per <<= 1;
+    // four logits per access where every lane's experts begin on a multiple of four of an aligned row
+    const int size = f32 ? 4 : 2;
+    const bool wide = p.gs % 4 == 0 && p.q % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) | uintptr_t(T > 1 ? ld * size : 0)) % (4 * size) == 0;
+    const int blocks = std::min((T + 3) / 4, 148 * 8);
+    auto go = [&](auto launcher) { launcher(f32, score, p, by_logit, top2, wide, blocks, st); };
     switch (per) {
-        case 1: launch<1>(f32, score, p, by_logit, top2, st); break;
-        case 2: launch<2>(f32, score, p, by_logit, top2, st); break;
-        case 4: launch<4>(f32, score, p, by_logit, top2, st); break;
-        case 8: launch<8>(f32, score, p, by_logit, top2, st); break;
-        case 16: launch<16>(f32, score, p, by_logit, top2, st); break;
-        case 32: launch<32>(f32, score, p, by_logit, top2, st); break;
-        default: launch<64>(f32, score, p, by_logit, top2, st); break;   // up to 1024 experts: q <= 64
+        case 1: go(launch<1>); break;
+        case 2: go(launch<2>); break;
+        case 4: go(launch<4>); break;
+        case 8: go(launch<8>); break;
+        case 16: go(launch<16>); break;
+        case 32: go(launch<32>); break;
+        default: go(launch<64>); break;   // up to 1024 experts: q <= 64
     }
     return "k_moe_route<" + std::to_string(per) + "," + (f32 ? "float" : "half") + "," + (score == kSigmoid ? "sigmoid" : "softmax") + "> grid=" +
-           std::to_string((T + 3) / 4);
+           std::to_string(blocks);
 }
 
 }  // namespace berth
