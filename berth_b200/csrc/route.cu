@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 namespace berth {
 namespace {
@@ -151,34 +152,41 @@ __device__ __forceinline__ float rcp(float x) { float y; asm("rcp.approx.ftz.f32
 
 // One warp per token; lane = P lanes per group, q consecutive experts each.
 //
-// The choice is made in 32 bits first and in 64 only where that cannot tell: an expert's key is the order of its fp32 choice
-// score with the lowest log2(PER) bits replaced by its place in the lane, a lane keeps its keys sorted, and a round takes the
-// largest head of the 32 lanes (one redux, one ballot).  Where two neighbours in the order, the first expert not chosen among them,
-// or the last group kept and the first one dropped, lie closer than both scores' errors, the warp repeats the choice in 64 bits.
+// The choice is made in 32 bits first and repeated in 64 (choose64) where that cannot tell.  An expert's key is its choice score in
+// fixed point with its place, (31 - lane, PER - 1 - i), in the lowest bits: keys differ, the larger key is the larger score or of
+// equal ones the lower expert, and a round of the choice is one redux over the lanes' heads.  A lane keeps its keys sorted.
+//   scores + bias: 2^QB steps over [least bias, 1 + largest bias];  fp32 logits by themselves: over the 32 below the row's largest;
+//   fp16 logits by themselves: the order of their bits, which have room for the place: exact.
+// Where two neighbours in the order (the first expert not chosen among them), or the last group kept and the first one dropped, lie
+// closer than both scores' errors and the steps, the choice is repeated; so it is for a row that has an infinite or NaN logit.
 // Errors of c = s + b in units of 2^-24: sigmoid, s (1 - s) (1.5 |l| + 4) for exp and 3 for sum and reciprocal, below 4.5 each;
 // softmax, s (2.5 |l - m| + 7) <= 9 each and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below 2 (28 + PER) for a pair; the sum
-// with the bias |c|; the place bits 2 PER |c|.  fp16 logits ordered by themselves lose nothing to the place bits: never repeated.
-template <int PER, bool F32, int SCORE>   // SCORE: kSigmoid or kSoftmax
-__global__ void __launch_bounds__(128) k_moe_route(const RouteParams p, bool by_logit, bool top2, bool wide)
+// with the bias, and the bias less the least, half a step of at most the span each.
+// Bound: instructions (some 27 an expert of a lane).  16384 tokens of 256 experts, 8 groups: %%
+template <int PER> struct Log2 { static constexpr int v = 1 + Log2<PER / 2>::v; };
+template <> struct Log2<1> { static constexpr int v = 0; };
+
+template <int PER, bool F32, int ORDER>
+__global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_route(const RouteParams p, bool sigmoid, bool top2, bool wide)
 {
-    constexpr unsigned kMask = PER - 1;
-    constexpr bool kSorted = PER <= 8;
-    constexpr float kLog2e = 1.44269504088896341f, kUnit = 1.f / (1 << 24);
-    __shared__ uint2 chosen[4][33];
+    constexpr int kPlace = 5 + Log2<PER>::v, kSteps = 32 - kPlace < 23 ? 32 - kPlace : 23;
+    constexpr unsigned kMask = (1u << kPlace) - 1;
+    constexpr bool kSorted = PER <= 8, kExact = ORDER == kByLogit && !F32, kHeldBias = PER <= 16 && ORDER != kByLogit, kAhead = PER <= 16;
+    constexpr float kLog2e = 1.44269504088896341f, kUnit = 1.f / (1 << 24), kMagic = 8388608.f;   // 2^23 + n: n in the low bits
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int g = lane / p.P, first = (lane % p.P) * p.q;
+    const int lane = threadIdx.x & 31;
+    const int log_p = 31 - __clz(p.P), g = lane >> log_p, first = (lane & (p.P - 1)) * p.q;
     const int cnt = g < p.G ? min(max(p.gs - first, 0), p.q) : 0;
     const int base = g < p.G ? g * p.gs + first : 0;
-    const float tol = by_logit ? (F32 ? 0.f : -1.f) : kUnit * (SCORE == kSigmoid ? 9.f : 2.f * (28 + PER));
-    const float tol_rel = by_logit ? 0.f : kUnit * (2.f + 2.f * PER);
+    const bool full = __all_sync(dq::kFull, cnt == PER);
+    const bool groups = p.keep < p.G;
     auto fetch = [&](int t, float (&l)[PER]) {
         const char* row = static_cast<const char*>(p.logits) + size_t(t) * p.ld * (F32 ? 4 : 2);
         if (PER >= 4 && wide) {
 #pragma unroll
             for (int i = 0; i < PER; i += 4) {
-                float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float v[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};
                 if (i < cnt) {
                     if constexpr (F32) {
                         const float4 w = *reinterpret_cast<const float4*>(row + size_t(base + i) * 4);
@@ -194,62 +202,101 @@ __global__ void __launch_bounds__(128) k_moe_route(const RouteParams p, bool by_
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) l[i] = i < cnt ? (F32 ? reinterpret_cast<const float*>(row)[base + i] : __half2float(reinterpret_cast<const __half*>(row)[base + i])) : -INFINITY;
+            for (int i = 0; i < PER; ++i)
+                l[i] = i < cnt ? (F32 ? reinterpret_cast<const float*>(row)[base + i] : __half2float(reinterpret_cast<const __half*>(row)[base + i])) : -FLT_MAX;
         }
     };
-    const int stride = gridDim.x * 4;
-    float next[PER];
-    int t = blockIdx.x * 4 + warp;
-    if (t < p.T) fetch(t, next);
-    for (; t < p.T; t += stride) {
-        const char* row = static_cast<const char*>(p.logits) + size_t(t) * p.ld * (F32 ? 4 : 2);
-        float l[PER];
-        bool nan = false;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            l[i] = clamp_logit(next[i]);
-            nan |= l[i] != l[i];
-        }
-        if (t + stride < p.T) fetch(t + stride, next);
 
-        // ---- choice scores in fp32
-        float m = -INFINITY, z = 0.f;   // softmax over all experts
-        const bool whole = SCORE == kSoftmax && (!by_logit || !p.renorm);
-        if (whole) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) m = fmaxf(m, l[i]);
-            m = redux_max(m);
-        }
-        float c[PER];
+    // the bias and its range
+    float bias[kHeldBias ? PER : 1];
+    float low = 0.f, span = 1.f;
+    if (ORDER != kByLogit && p.bias) {
+        float lo = INFINITY, hi = -INFINITY;
+        bool odd = false;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            c[i] = l[i];
-            if (SCORE == kSigmoid) {
-                if (!by_logit && l[i] > -INFINITY) c[i] = rcp(1.f + ex2(-l[i] * kLog2e));
-            } else if (whole) {
-                const float e = l[i] > -INFINITY ? ex2((l[i] - m) * kLog2e) : 0.f;
-                z += e;
-                if (!by_logit && l[i] > -INFINITY) c[i] = e;
+            const float b = i < cnt ? p.bias[base + i] : 0.f;
+            if constexpr (kHeldBias) bias[i] = b;
+            if (i < cnt) {
+                lo = fminf(lo, b);
+                hi = fmaxf(hi, b);
+                odd |= !(fabsf(b) < 1e30f);
             }
         }
-        if (whole) z = warp_sum(z);
-        if (!by_logit) {
-            const float inv = SCORE == kSoftmax ? rcp(z) : 1.f;
+        low = redux_min(lo);
+        span = 1.f + (redux_max(hi) - low);
+        if constexpr (kHeldBias) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (i < cnt && l[i] > -INFINITY) {
-                    if (SCORE == kSoftmax) c[i] *= inv;
-                    if (p.bias) c[i] += p.bias[base + i];
-                }
+            for (int i = 0; i < PER; ++i) bias[i] -= low;   // scores from 0 on: the order is the same
         }
+        if (__any_sync(dq::kFull, odd)) span = INFINITY;   // every row in 64 bits
+    } else if constexpr (kHeldBias) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) bias[i] = 0.f;
+    }
+    if (ORDER == kByLogit) span = 32.f;
+    const bool never = !(span < 1e30f);
+    const float scale = ((1 << kSteps) - 4) / span;
+    // how close two choice scores, or two groups' scores, may lie before 64 bits decide: their errors, and two steps of each key
+    const float error = ORDER == kByLogit ? 0.f : kUnit * ((ORDER == kSigmoid ? 9.f : 2.f * (28 + PER)) + 4.f * span);
+    const unsigned near = kExact ? 0u : unsigned(error * scale) + 4u;
 
-        // ---- groups
-        bool unsure = false, dropped = false;
-        if (p.keep < p.G) {
-            float b1 = -INFINITY, b2 = -INFINITY;
+    const int stride = gridDim.x * 4;
+    float next[kAhead ? PER : 1];
+    int t = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if constexpr (kAhead) {
+        if (t < p.T) fetch(t, next);
+    }
+    for (; t < p.T; t += stride) {
+        const char* row = static_cast<const char*>(p.logits) + size_t(t) * p.ld * (F32 ? 4 : 2);
+        float l[PER], c[PER];
+        bool unsure = never;
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) l[i] = next[i];
+            if (t + stride < p.T) fetch(t + stride, next);
+        } else fetch(t, l);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) unsure |= !(fabsf(l[i]) <= FLT_MAX);
+
+        // ---- choice scores
+        float m = 0.f, z = 0.f;
+        if (ORDER == kSoftmax || (ORDER == kByLogit && (F32 || !(sigmoid || p.renorm)))) {
+            m = l[0];
+#pragma unroll
+            for (int i = 1; i < PER; ++i) m = fmaxf(m, l[i]);
+            m = redux_max(m);
+        }
+        if (ORDER == kSoftmax || (ORDER == kByLogit && !(sigmoid || p.renorm))) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                b2 = fmaxf(b2, fminf(b1, c[i]));   // (NaN: neither changes; a padded place is -inf)
+                c[i] = full || i < cnt ? ex2((l[i] - m) * kLog2e) : 0.f;
+                z += c[i];
+            }
+            z = warp_sum(z);
+        }
+        const float inv = ORDER == kSoftmax ? rcp(z) : 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (ORDER == kByLogit) c[i] = l[i];
+            else if (ORDER == kSigmoid) c[i] = rcp(1.f + ex2(l[i] * -kLog2e));
+            else c[i] *= inv;
+            if constexpr (kHeldBias) c[i] += bias[i];
+            else if (ORDER != kByLogit && p.bias && i < cnt) c[i] += p.bias[base + i] - low;
+        }
+        if (!full) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (i >= cnt) c[i] = -FLT_MAX;
+        }
+
+        // ---- groups: rounds over the lanes' (their groups') scores
+        bool open = g < p.G;
+        if (groups) {
+            float b1 = c[0], b2 = -FLT_MAX;
+#pragma unroll
+            for (int i = 1; i < PER; ++i) {
+                b2 = fmaxf(b2, fminf(b1, c[i]));
                 b1 = fmaxf(b1, c[i]);
             }
             for (int off = 1; off < p.P; off <<= 1) {
@@ -257,35 +304,51 @@ __global__ void __launch_bounds__(128) k_moe_route(const RouteParams p, bool by_
                 b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
                 b1 = fmaxf(b1, o1);
             }
-            const float score = top2 && b2 > -INFINITY ? b1 + b2 : b1;
-            int before = 0;
-            for (int j = 0; j < p.G; ++j) {
-                const float o = __shfl_sync(dq::kFull, score, j * p.P);
-                before += o > score || (o == score && j < g);
+            float score = open ? (top2 ? b1 + b2 : b1) : -INFINITY, top = 0.f;
+            open = false;
+            for (int s = 0; s < p.keep; ++s) {
+                top = redux_max(score);
+                const int winner = (__ffs(__ballot_sync(dq::kFull, score == top)) - 1) >> log_p;
+                if (g == winner) {
+                    open = true;
+                    score = -INFINITY;
+                }
             }
-            dropped = before >= p.keep;
-            const float least = redux_min(g < p.G && !dropped ? score : INFINITY), most = redux_max(g < p.G && dropped ? score : -INFINITY);
-            const float size = redux_max(b1 > -INFINITY ? fabsf(b1) + (b2 > -INFINITY ? fabsf(b2) : 0.f) : 0.f);   // what the sums' roundings scale with
-            unsure = least - most <= (by_logit ? -1.f : 2.f * tol + tol_rel * size);
+            if (ORDER != kByLogit) unsure |= top - redux_max(score) <= 2.f * error;
         }
 
         // ---- keys, largest first
         unsigned key[PER];
+        const unsigned place = (31u - lane) << Log2<PER>::v;
+        const float shift = ORDER == kByLogit ? kMagic + float((1 << kSteps) - 3) : kMagic + 1.f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const unsigned b = __float_as_uint(c[i] + 0.f);
-            const unsigned o = c[i] != c[i] ? 0x80u : ((b >> 31) ? ~b : b | 0x80000000u);
-            key[i] = i < cnt && !dropped ? (o & ~kMask) | (kMask - i) : 0u;
+            if constexpr (kExact) {
+                const int b = __float_as_int(c[i] + 0.f);
+                key[i] = ((unsigned(b) ^ (unsigned(b >> 31) | 0x80000000u)) & ~kMask) | place | unsigned(PER - 1 - i);
+            } else {
+                const float n = ORDER == kByLogit ? fmaxf(fmaf(c[i] - m, scale, shift), kMagic) : fmaf(c[i], scale, shift);
+                key[i] = ((__float_as_uint(n) & ((1u << kSteps) - 1)) << kPlace) | place | unsigned(PER - 1 - i);
+            }
+        }
+        if (!full) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (i >= cnt) key[i] = 0;
+        }
+        if (!open) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) key[i] = 0;
         }
         if constexpr (kSorted && PER > 1) {
 #pragma unroll
-            for (int span = 2; span <= PER; span *= 2)      // bitonic, descending
+            for (int span = 2; span <= PER; span *= 2)      // bitonic, descending; the first step of a span is mirrored
 #pragma unroll
                 for (int d = span / 2; d >= 1; d /= 2)
 #pragma unroll
                     for (int i = 0; i < PER; ++i)
                         if (!(i & d)) {
-                            const int j = d == span / 2 ? (i | (span - 1)) - (i & (span / 2 - 1)) : i + d;   // first step of a span: mirrored
+                            const int j = d == span / 2 ? (i | (span - 1)) - (i & (span / 2 - 1)) : i + d;
                             const unsigned hi = max(key[i], key[j]), lo = min(key[i], key[j]);
                             key[i] = hi;
                             key[j] = lo;
@@ -296,39 +359,54 @@ __global__ void __launch_bounds__(128) k_moe_route(const RouteParams p, bool by_
 #pragma unroll
             for (int i = 1; i < PER; ++i) head = max(head, key[i]);
         }
-        for (int s = 0; s <= p.k; ++s) {     // one more than is chosen: the first that is not
-            const unsigned top = __reduce_max_sync(dq::kFull, head & ~kMask);
-            const int owner = __ffs(__ballot_sync(dq::kFull, (head & ~kMask) == top)) - 1;
-            if (lane == owner) {
-                chosen[warp][s] = make_uint2(unsigned(base) + (kMask - (head & kMask)), top);
-                if constexpr (kSorted) {
+        unsigned won = 0, after = 0;     // lane s: the s-th key, and the next one
+        for (int s = 0; s <= p.k; ++s) {
+            const unsigned top = __reduce_max_sync(dq::kFull, head);
+            if (lane == s) won = top;
+            if (lane + 1 == s) after = top;
+            if constexpr (kSorted) {
+                const bool mine = head == top;
 #pragma unroll
-                    for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1];
-                    key[PER - 1] = 0;
-                    head = key[0];
-                } else {
-                    unsigned h = 0;
+                for (int i = 0; i + 1 < PER; ++i) key[i] = mine ? key[i + 1] : key[i];
+                key[PER - 1] = mine ? 0u : key[PER - 1];
+                head = key[0];
+            } else if (head == top) {
+                unsigned h = 0;
 #pragma unroll
-                    for (int i = 0; i < PER; ++i) {
-                        key[i] = key[i] == head ? 0u : key[i];
-                        h = max(h, key[i]);
-                    }
-                    head = h;
+                for (int i = 0; i < PER; ++i) {
+                    key[i] = key[i] == head ? 0u : key[i];
+                    h = max(h, key[i]);
                 }
+                head = h;
             }
         }
-        __syncwarp();
-        int mine = 0;
-        if (lane < p.k) {
-            const uint2 a = chosen[warp][lane], b = chosen[warp][lane + 1];
-            auto value = [](unsigned o) { return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o); };   // below -FLT_MAX: NaN, which is never unsure
-            const float va = value(a.y), vb = value(b.y);
-            mine = int(a.x);
-            unsure |= b.y != 0u && va - vb <= tol + tol_rel * fmaxf(fabsf(va), fabsf(vb));
+        if (!kExact) unsure |= lane < p.k && after != 0u && (won >> kPlace) - (after >> kPlace) <= near;
+        // (below the 32 of the logits, the steps end)
+        if (ORDER == kByLogit && F32) unsure |= lane < p.k && (won >> kPlace) <= 4u;
+        const int owner = 31 - int(won >> Log2<PER>::v & 31u);
+        int mine = (owner >> log_p) * p.gs + (owner & (p.P - 1)) * p.q + (PER - 1 - int(won & (PER - 1)));
+        const bool again = __any_sync(dq::kFull, unsure);
+        bool nan = false;
+        if (again) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                nan |= l[i] != l[i];
+                l[i] = clamp_logit(l[i]);
+            }
+            nan = __any_sync(dq::kFull, nan);
+            mine = choose64<PER>(l, cnt, base, ORDER, top2, p);
+            if (!(sigmoid || p.renorm)) {   // softmax over the row as it is, masked experts left out
+                m = -INFINITY;
+                z = 0.f;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) m = i < cnt ? fmaxf(m, l[i]) : m;
+                m = redux_max(m);
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (i < cnt && l[i] > -INFINITY) z += ex2((l[i] - m) * kLog2e);
+                z = warp_sum(z);
+            }
         }
-        __syncwarp();
-        if (__any_sync(dq::kFull, unsure)) mine = choose64<PER>(l, cnt, base, by_logit ? kByLogit : SCORE, top2, p);
-        nan = __any_sync(dq::kFull, nan);
 
         // ---- the weight of this lane's expert
         const float v = lane < p.k ? logit_at<F32>(row, mine) : -INFINITY;
@@ -336,29 +414,36 @@ __global__ void __launch_bounds__(128) k_moe_route(const RouteParams p, bool by_
         if (p.renorm) {
             const float most = redux_max(v);
             // relative to the largest of the chosen; a sigmoid far below zero is exp of its logit (within 2^-43)
-            if (SCORE == kSoftmax || most < -30.f) w = v > -INFINITY ? expf(v - most) : 0.f;
-            else w = 1.f / (1.f + expf(-v));
+            if (!sigmoid || most < -30.f) w = v > -INFINITY ? expf(v - most) : 0.f;
+            else w = __fdividef(1.f, 1.f + expf(-v));
             if (lane >= p.k) w = 0.f;
             const float sum = warp_sum(w);
-            w = sum > 0.f ? w / sum : 0.f;
-        } else if (SCORE == kSigmoid) {
-            w = 1.f / (1.f + expf(-v));
+            w = sum > 0.f ? __fdividef(w, sum) : 0.f;
+        } else if (sigmoid) {
+            w = __fdividef(1.f, 1.f + expf(-v));
         } else {
-            w = v > -INFINITY ? expf(v - m) / z : 0.f;
+            w = v > -INFINITY ? __fdividef(expf(v - m), z) : 0.f;
         }
         if (lane < p.k) {
-            p.idx[size_t(t) * p.k + lane] = mine;
-            p.w[size_t(t) * p.k + lane] = nan ? NAN : w * p.scale;
+            const size_t at = size_t(t) * p.k + lane;
+            p.idx[at] = mine;
+            p.w[at] = nan ? NAN : w * p.scale;
         }
     }
 }
 
 template <int PER>
-void launch(bool f32, int score, const RouteParams& p, bool by_logit, bool top2, bool wide, int blocks, cudaStream_t st)
+void launch(bool f32, int order, bool sigmoid, const RouteParams& p, bool top2, bool wide, int blocks, cudaStream_t st)
 {
-    auto go = [&](auto kern) { launch_pdl(kern, dim3(blocks), dim3(128), 0, st, "k_moe_route launch", p, by_logit, top2, wide); };
-    if (f32) score == kSigmoid ? go(k_moe_route<PER, true, kSigmoid>) : go(k_moe_route<PER, true, kSoftmax>);
-    else score == kSigmoid ? go(k_moe_route<PER, false, kSigmoid>) : go(k_moe_route<PER, false, kSoftmax>);
+    auto go = [&](auto kern) { launch_pdl(kern, dim3(blocks), dim3(128), 0, st, "k_moe_route launch", p, sigmoid, top2, wide); };
+    auto typed = [&](auto f) {
+        constexpr bool F = decltype(f)::value;
+        if (order == kByLogit) go(k_moe_route<PER, F, kByLogit>);
+        else if (order == kSigmoid) go(k_moe_route<PER, F, kSigmoid>);
+        else go(k_moe_route<PER, F, kSoftmax>);
+    };
+    if (f32) typed(std::true_type{});
+    else typed(std::false_type{});
 }
 
 }  // namespace
@@ -399,7 +484,7 @@ std::string route_tokens(const void* logits, bool f32, long long ld, const berth
     const int size = f32 ? 4 : 2;
     const bool wide = p.gs % 4 == 0 && p.q % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) | uintptr_t(T > 1 ? ld * size : 0)) % (4 * size) == 0;
     const int blocks = std::min((T + 3) / 4, 148 * 8);
-    auto go = [&](auto launcher) { launcher(f32, score, p, by_logit, top2, wide, blocks, st); };
+    auto go = [&](auto launcher) { launcher(f32, by_logit ? kByLogit : score, score == kSigmoid, p, top2, wide, blocks, st); };
     switch (per) {
         case 1: go(launch<1>); break;
         case 2: go(launch<2>); break;
@@ -409,7 +494,7 @@ std::string route_tokens(const void* logits, bool f32, long long ld, const berth
         case 32: go(launch<32>); break;
         default: go(launch<64>); break;   // up to 1024 experts: q <= 64
     }
-    return "k_moe_route<" + std::to_string(per) + "," + (f32 ? "float" : "half") + "," + (score == kSigmoid ? "sigmoid" : "softmax") + "> grid=" +
+    return "k_moe_route<" + std::to_string(per) + "," + (f32 ? "float" : "half") + "," + (score == kSigmoid ? "sigmoid" : "softmax") + (by_logit ? "" : ",scores") + "> grid=" +
            std::to_string(blocks);
 }
 
