@@ -163,6 +163,13 @@ __device__ __forceinline__ float rcp(float x) { float y; asm("rcp.approx.ftz.f32
 // softmax, s (2.5 |l - m| + 7) <= 9 each and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below 2 (28 + PER) for a pair; the sum
 // with the bias, and the bias less the least, half a step of at most the span each.
 // Bound: instructions (some 27 an expert of a lane).  16384 tokens of 256 experts, 8 groups: %%
+// The order of a finite float's bits (-0 as +0).
+__device__ __forceinline__ unsigned ordered(float v)
+{
+    const int b = __float_as_int(v + 0.f);
+    return unsigned(b) ^ (unsigned(b >> 31) | 0x80000000u);
+}
+
 template <int PER> struct Log2 { static constexpr int v = 1 + Log2<PER / 2>::v; };
 template <> struct Log2<1> { static constexpr int v = 0; };
 
@@ -173,9 +180,11 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
     constexpr unsigned kMask = (1u << kPlace) - 1;
     constexpr bool kSorted = PER <= 8, kExact = ORDER == kByLogit && !F32, kHeldBias = PER <= 16 && ORDER != kByLogit, kAhead = PER <= 16;
     constexpr float kLog2e = 1.44269504088896341f, kUnit = 1.f / (1 << 24), kMagic = 8388608.f;   // 2^23 + n: n in the low bits
+    __shared__ __align__(16) unsigned sorted[4][kSorted ? 32 * PER : 1];   // every lane's keys
+    __shared__ unsigned winners[4][33];
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int log_p = 31 - __clz(p.P), g = lane >> log_p, first = (lane & (p.P - 1)) * p.q;
     const int cnt = g < p.G ? min(max(p.gs - first, 0), p.q) : 0;
     const int base = g < p.G ? g * p.gs + first : 0;
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
 
     const int stride = gridDim.x * 4;
     float next[kAhead ? PER : 1];
-    int t = blockIdx.x * 4 + (threadIdx.x >> 5);
+    int t = blockIdx.x * 4 + warp;
     if constexpr (kAhead) {
         if (t < p.T) fetch(t, next);
     }
@@ -304,17 +313,22 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
                 b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
                 b1 = fmaxf(b1, o1);
             }
-            float score = open ? (top2 ? b1 + b2 : b1) : -INFINITY, top = 0.f;
+            const float score = top2 ? b1 + b2 : b1;
+            unsigned gkey, top = 0;
+            if constexpr (kExact) gkey = ordered(score) & ~31u;
+            else if constexpr (ORDER == kByLogit) gkey = __float_as_uint(fmaxf(fmaf(score - m, scale, kMagic + float((1 << kSteps) - 3)), kMagic)) << 5;
+            else gkey = __float_as_uint(fmaf(score, 0.5f * scale, kMagic + 1.f)) << 5;
+            gkey = open ? gkey | (31u - g) : 0u;
             open = false;
             for (int s = 0; s < p.keep; ++s) {
-                top = redux_max(score);
-                const int winner = (__ffs(__ballot_sync(dq::kFull, score == top)) - 1) >> log_p;
-                if (g == winner) {
+                top = __reduce_max_sync(dq::kFull, gkey);
+                if (gkey == top) {
                     open = true;
-                    score = -INFINITY;
+                    gkey = 0;
                 }
             }
-            if (ORDER != kByLogit) unsure |= top - redux_max(score) <= 2.f * error;
+            if (!kExact) unsure |= (top >> 5) - (__reduce_max_sync(dq::kFull, gkey) >> 5) <= near;
+            if (ORDER == kByLogit && F32) unsure |= (top >> 5 & ((1u << kSteps) - 1)) <= 4u;   // (below the 32 of the logits, the steps end)
         }
 
         // ---- keys, largest first
@@ -324,11 +338,10 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if constexpr (kExact) {
-                const int b = __float_as_int(c[i] + 0.f);
-                key[i] = ((unsigned(b) ^ (unsigned(b >> 31) | 0x80000000u)) & ~kMask) | place | unsigned(PER - 1 - i);
+                key[i] = (ordered(c[i]) & ~kMask) | place | unsigned(PER - 1 - i);
             } else {
                 const float n = ORDER == kByLogit ? fmaxf(fmaf(c[i] - m, scale, shift), kMagic) : fmaf(c[i], scale, shift);
-                key[i] = ((__float_as_uint(n) & ((1u << kSteps) - 1)) << kPlace) | place | unsigned(PER - 1 - i);
+                key[i] = __float_as_uint(n) << kPlace | place | unsigned(PER - 1 - i);   // (what the exponent leaves is the same in all)
             }
         }
         if (!full) {
@@ -355,34 +368,47 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
                         }
         }
         unsigned head = key[0];
-        if constexpr (!kSorted) {
+        if constexpr (kSorted) {
+            // the keys to shared memory: the owner of a round's key reads its next one, instead of moving all of them up
+            unsigned* place_of = &sorted[warp][lane * PER];
+            if constexpr (PER % 4 == 0) {
+#pragma unroll
+                for (int i = 0; i < PER; i += 4) *reinterpret_cast<uint4*>(place_of + i) = make_uint4(key[i], key[(i + 1) % PER], key[(i + 2) % PER], key[(i + 3) % PER]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) place_of[i] = key[i];
+            }
+            int left = PER - 1;
+            for (int s = 0; s <= p.k; ++s) {
+                const unsigned top = __reduce_max_sync(dq::kFull, head);
+                if (head == top) {
+                    winners[warp][s] = top;
+                    ++place_of;
+                    head = left-- > 0 ? *place_of : 0u;
+                }
+            }
+        } else {
 #pragma unroll
             for (int i = 1; i < PER; ++i) head = max(head, key[i]);
-        }
-        unsigned won = 0, after = 0;     // lane s: the s-th key, and the next one
-        for (int s = 0; s <= p.k; ++s) {
-            const unsigned top = __reduce_max_sync(dq::kFull, head);
-            if (lane == s) won = top;
-            if (lane + 1 == s) after = top;
-            if constexpr (kSorted) {
-                const bool mine = head == top;
+            for (int s = 0; s <= p.k; ++s) {
+                const unsigned top = __reduce_max_sync(dq::kFull, head);
+                if (head == top) {
+                    winners[warp][s] = top;
+                    unsigned h = 0;
 #pragma unroll
-                for (int i = 0; i + 1 < PER; ++i) key[i] = mine ? key[i + 1] : key[i];
-                key[PER - 1] = mine ? 0u : key[PER - 1];
-                head = key[0];
-            } else if (head == top) {
-                unsigned h = 0;
-#pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    key[i] = key[i] == head ? 0u : key[i];
-                    h = max(h, key[i]);
+                    for (int i = 0; i < PER; ++i) {
+                        key[i] = key[i] == head ? 0u : key[i];
+                        h = max(h, key[i]);
+                    }
+                    head = h;
                 }
-                head = h;
             }
         }
+        __syncwarp();
+        const unsigned won = winners[warp][lane], after = winners[warp][lane + 1];   // of lane s < k: the s-th key, and the next
+        __syncwarp();
         if (!kExact) unsure |= lane < p.k && after != 0u && (won >> kPlace) - (after >> kPlace) <= near;
-        // (below the 32 of the logits, the steps end)
-        if (ORDER == kByLogit && F32) unsure |= lane < p.k && (won >> kPlace) <= 4u;
+        if (ORDER == kByLogit && F32) unsure |= lane < p.k && (won >> kPlace & ((1u << kSteps) - 1)) <= 4u;
         const int owner = 31 - int(won >> Log2<PER>::v & 31u);
         int mine = (owner >> log_p) * p.gs + (owner & (p.P - 1)) * p.q + (PER - 1 - int(won & (PER - 1)));
         const bool again = __any_sync(dq::kFull, unsure);
@@ -417,7 +443,8 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
             if (!sigmoid || most < -30.f) w = v > -INFINITY ? expf(v - most) : 0.f;
             else w = __fdividef(1.f, 1.f + expf(-v));
             if (lane >= p.k) w = 0.f;
-            const float sum = warp_sum(w);
+            float sum = w;
+            for (int off = 1; off < p.k; off <<= 1) sum += __shfl_xor_sync(dq::kFull, sum, off);   // (lanes from k on: 0)
             w = sum > 0.f ? __fdividef(w, sum) : 0.f;
         } else if (sigmoid) {
             w = __fdividef(1.f, 1.f + expf(-v));
