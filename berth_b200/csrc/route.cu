@@ -61,7 +61,7 @@ __device__ __forceinline__ float warp_sum(float v)
 // The choice with every score and comparison in 64 bits.  Lane s returns the s-th chosen expert.  The experts of a lane
 // are consecutive and rise with the lane, so the first lane and the first of its experts have the lower index of a tie.
 template <int PER>
-__device__ __noinline__ int choose64(const float (&l)[PER], int cnt, int base, int order, bool top2, const RouteParams& p)
+__device__ __forceinline__ int choose64(const float (&l)[PER], int cnt, int base, int order, bool top2, const RouteParams& p)
 {
     const int lane = threadIdx.x & 31;
     double c[PER];
@@ -163,6 +163,35 @@ __device__ __forceinline__ float rcp(float x) { float y; asm("rcp.approx.ftz.f32
 // softmax, s (2.5 |l - m| + 7) <= 9 each and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below 2 (28 + PER) for a pair; the sum
 // with the bias, and the bias less the least, half a step of at most the span each.
 // Bound: instructions (some 27 an expert of a lane).  16384 tokens of 256 experts, 8 groups: %%
+// A row whose choice 32 bits cannot tell, or with an infinite or NaN logit: its logits once more, the choice in 64 bits, and what a
+// softmax over the row needs.
+struct Again {
+    int mine;
+    bool nan;
+    float m, z;
+};
+template <int PER, bool F32>
+__device__ __noinline__ Again choose_again(const char* row, int cnt, int base, int order, bool top2, bool softmax, const RouteParams& p)
+{
+    float l[PER], m = -INFINITY, z = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        l[i] = i < cnt ? logit_at<F32>(row, base + i) : -INFINITY;
+        nan |= l[i] != l[i];
+        m = fmaxf(m, l[i]);
+    }
+    m = redux_max(m);
+    if (softmax) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (l[i] > -INFINITY) z += ex2((l[i] - m) * 1.44269504088896341f);
+        z = warp_sum(z);
+    }
+    nan = __any_sync(dq::kFull, nan);
+    return Again{choose64<PER>(l, cnt, base, order, top2, p), nan, m, z};
+}
+
 // The order of a finite float's bits (-0 as +0).
 __device__ __forceinline__ unsigned ordered(float v)
 {
@@ -177,10 +206,11 @@ template <int PER, bool F32, int ORDER>
 __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_route(const RouteParams p, bool sigmoid, bool top2, bool wide)
 {
     constexpr int kPlace = 5 + Log2<PER>::v, kSteps = 32 - kPlace < 23 ? 32 - kPlace : 23;
+    constexpr int kRoom = PER + 4;   // words of a lane's keys, the last of them 0
     constexpr unsigned kMask = (1u << kPlace) - 1;
     constexpr bool kSorted = PER <= 8, kExact = ORDER == kByLogit && !F32, kHeldBias = PER <= 16 && ORDER != kByLogit, kAhead = PER <= 16;
     constexpr float kLog2e = 1.44269504088896341f, kUnit = 1.f / (1 << 24), kMagic = 8388608.f;   // 2^23 + n: n in the low bits
-    __shared__ __align__(16) unsigned sorted[4][kSorted ? 32 * PER : 1];   // every lane's keys
+    __shared__ __align__(16) unsigned sorted[4][kSorted ? 32 * kRoom : 4];   // every lane's keys
     __shared__ unsigned winners[4][33];
     pdl_trigger();
     pdl_wait();
@@ -250,6 +280,7 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
     const float error = ORDER == kByLogit ? 0.f : kUnit * ((ORDER == kSigmoid ? 9.f : 2.f * (28 + PER)) + 4.f * span);
     const unsigned near = kExact ? 0u : unsigned(error * scale) + 4u;
 
+    if constexpr (kSorted) sorted[warp][lane * kRoom + PER] = 0;
     const int stride = gridDim.x * 4;
     float next[kAhead ? PER : 1];
     int t = blockIdx.x * 4 + warp;
@@ -369,23 +400,26 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
         }
         unsigned head = key[0];
         if constexpr (kSorted) {
-            // the keys to shared memory: the owner of a round's key reads its next one, instead of moving all of them up
-            unsigned* place_of = &sorted[warp][lane * PER];
+            // the keys to shared memory, a 0 behind them: the owner of a round's key reads its next one, instead of moving all up
+            unsigned* mine_at = &sorted[warp][lane * kRoom];
             if constexpr (PER % 4 == 0) {
 #pragma unroll
-                for (int i = 0; i < PER; i += 4) *reinterpret_cast<uint4*>(place_of + i) = make_uint4(key[i], key[(i + 1) % PER], key[(i + 2) % PER], key[(i + 3) % PER]);
+                for (int i = 0; i < PER; i += 4) *reinterpret_cast<uint4*>(mine_at + i) = make_uint4(key[i], key[(i + 1) % PER], key[(i + 2) % PER], key[(i + 3) % PER]);
             } else {
 #pragma unroll
-                for (int i = 0; i < PER; ++i) place_of[i] = key[i];
+                for (int i = 0; i < PER; ++i) mine_at[i] = key[i];
             }
-            int left = PER - 1;
-            for (int s = 0; s <= p.k; ++s) {
+            uint32_t from = uint32_t(__cvta_generic_to_shared(mine_at)), to = uint32_t(__cvta_generic_to_shared(winners[warp]));
+            for (int s = 0; s <= p.k; ++s, to += 4) {
                 const unsigned top = __reduce_max_sync(dq::kFull, head);
-                if (head == top) {
-                    winners[warp][s] = top;
-                    ++place_of;
-                    head = left-- > 0 ? *place_of : 0u;
-                }
+                asm volatile("{\n\t.reg .pred q;\n\t"
+                             "setp.eq.u32 q, %0, %2;\n\t"
+                             "@q st.shared.u32 [%3], %2;\n\t"
+                             "@q add.u32 %1, %1, 4;\n\t"
+                             "@q ld.shared.u32 %0, [%1];\n\t}"
+                             : "+r"(head), "+r"(from)
+                             : "r"(top), "r"(to)
+                             : "memory");
             }
         } else {
 #pragma unroll
@@ -411,27 +445,13 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
         if (ORDER == kByLogit && F32) unsure |= lane < p.k && (won >> kPlace & ((1u << kSteps) - 1)) <= 4u;
         const int owner = 31 - int(won >> Log2<PER>::v & 31u);
         int mine = (owner >> log_p) * p.gs + (owner & (p.P - 1)) * p.q + (PER - 1 - int(won & (PER - 1)));
-        const bool again = __any_sync(dq::kFull, unsure);
         bool nan = false;
-        if (again) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                nan |= l[i] != l[i];
-                l[i] = clamp_logit(l[i]);
-            }
-            nan = __any_sync(dq::kFull, nan);
-            mine = choose64<PER>(l, cnt, base, ORDER, top2, p);
-            if (!(sigmoid || p.renorm)) {   // softmax over the row as it is, masked experts left out
-                m = -INFINITY;
-                z = 0.f;
-#pragma unroll
-                for (int i = 0; i < PER; ++i) m = i < cnt ? fmaxf(m, l[i]) : m;
-                m = redux_max(m);
-#pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    if (i < cnt && l[i] > -INFINITY) z += ex2((l[i] - m) * kLog2e);
-                z = warp_sum(z);
-            }
+        if (__any_sync(dq::kFull, unsure)) {
+            const Again o = choose_again<PER, F32>(row, cnt, base, ORDER, top2, !(sigmoid || p.renorm), p);
+            mine = o.mine;
+            nan = o.nan;
+            m = o.m;
+            z = o.z;
         }
 
         // ---- the weight of this lane's expert
