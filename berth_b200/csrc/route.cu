@@ -157,8 +157,9 @@ __device__ __forceinline__ float rcp(float x) { float y; asm("rcp.approx.ftz.f32
 // equal ones the lower expert, and a round of the choice is one redux over the lanes' heads.  A lane keeps its keys sorted.
 //   scores + bias: 2^QB steps over [least bias, 1 + largest bias];  fp32 logits by themselves: over the 32 below the row's largest;
 //   fp16 logits by themselves: the order of their bits, which have room for the place: exact.
-// Where two neighbours in the order (the first expert not chosen among them), or the last group kept and the first one dropped, lie
-// closer than both scores' errors and the steps, the choice is repeated; so it is for a row that has an infinite or NaN logit.
+// Where two neighbours in the order (the first expert not chosen among them) lie closer than both scores' errors and the steps, the
+// k + 1 first are ordered anew in 64 bits, one a lane; the whole choice is repeated where that may not be enough (a third one as
+// close, a softmax under a bias, the last group kept and the first one dropped as close) and for a row that has an infinite or NaN logit.
 // Errors of c = s + b in units of 2^-24: sigmoid, s (1 - s) (1.5 |l| + 4) for exp and 3 for sum and reciprocal, below 4.5 each;
 // softmax, s (2.5 |l - m| + 7) <= 9 each and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below 2 (28 + PER) for a pair; the sum
 // with the bias, and the bias less the least, half a step of at most the span each.
@@ -202,16 +203,20 @@ __device__ __forceinline__ unsigned ordered(float v)
 template <int PER> struct Log2 { static constexpr int v = 1 + Log2<PER / 2>::v; };
 template <> struct Log2<1> { static constexpr int v = 0; };
 
+// Blocks of an SM that the registers have to allow, and the grid fills once: eight keys a lane, 16384 tokens, 6: 16.0 us, 8: 17.3 us; two
+// keys a lane (64 experts) 8: 7.7 us, 6: 10.3 us.
+constexpr int min_blocks(int per) { return per < 8 ? 8 : per == 8 ? 6 : per == 16 ? 4 : 2; }
+
 template <int PER, bool F32, int ORDER>
-__global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_route(const RouteParams p, bool sigmoid, bool top2, bool wide)
+__global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteParams p, bool sigmoid, bool top2, bool wide)
 {
     constexpr int kPlace = 5 + Log2<PER>::v, kSteps = 32 - kPlace < 23 ? 32 - kPlace : 23;
-    constexpr int kRoom = PER + 4;   // words of a lane's keys, the last of them 0
+    constexpr int kRun = PER < 8 ? PER : 8, kRuns = PER / kRun, kRoom = (kRun + 4) * kRuns;   // a lane's keys: sorted runs, zeros behind each
     constexpr unsigned kMask = (1u << kPlace) - 1;
-    constexpr bool kSorted = PER <= 8, kExact = ORDER == kByLogit && !F32, kHeldBias = PER <= 16 && ORDER != kByLogit, kAhead = PER <= 16;
+    constexpr bool kSorted = PER <= 32, kExact = ORDER == kByLogit && !F32, kHeldBias = PER <= 16 && ORDER != kByLogit, kAhead = PER <= 16;
     constexpr float kLog2e = 1.44269504088896341f, kUnit = 1.f / (1 << 24), kMagic = 8388608.f;   // 2^23 + n: n in the low bits
     __shared__ __align__(16) unsigned sorted[4][kSorted ? 32 * kRoom : 4];   // every lane's keys
-    __shared__ unsigned winners[4][33];
+    __shared__ unsigned winners[4][34];
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -280,7 +285,10 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
     const float error = ORDER == kByLogit ? 0.f : kUnit * ((ORDER == kSigmoid ? 9.f : 2.f * (28 + PER)) + 4.f * span);
     const unsigned near = kExact ? 0u : unsigned(error * scale) + 4u;
 
-    if constexpr (kSorted) sorted[warp][lane * kRoom + PER] = 0;
+    if constexpr (kSorted) {
+        for (int r = 0; r < kRuns; ++r)
+            for (int i = 0; i < 4; ++i) sorted[warp][lane * kRoom + r * (kRun + 4) + kRun + i] = 0;   // (read once a round when no key is left)
+    }
     const int stride = gridDim.x * 4;
     float next[kAhead ? PER : 1];
     int t = blockIdx.x * 4 + warp;
@@ -386,45 +394,62 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
         }
         if constexpr (kSorted && PER > 1) {
 #pragma unroll
-            for (int span = 2; span <= PER; span *= 2)      // bitonic, descending; the first step of a span is mirrored
+            for (int r = 0; r < PER; r += kRun)
 #pragma unroll
-                for (int d = span / 2; d >= 1; d /= 2)
+                for (int span = 2; span <= kRun; span *= 2)      // bitonic, descending; the first step of a span is mirrored
 #pragma unroll
-                    for (int i = 0; i < PER; ++i)
-                        if (!(i & d)) {
-                            const int j = d == span / 2 ? (i | (span - 1)) - (i & (span / 2 - 1)) : i + d;
-                            const unsigned hi = max(key[i], key[j]), lo = min(key[i], key[j]);
-                            key[i] = hi;
-                            key[j] = lo;
-                        }
+                    for (int d = span / 2; d >= 1; d /= 2)
+#pragma unroll
+                        for (int i = 0; i < kRun; ++i)
+                            if (!(i & d)) {
+                                const int j = d == span / 2 ? (i | (span - 1)) - (i & (span / 2 - 1)) : i + d;
+                                const unsigned hi = max(key[r + i], key[r + j]), lo = min(key[r + i], key[r + j]);
+                                key[r + i] = hi;
+                                key[r + j] = lo;
+                            }
         }
         unsigned head = key[0];
         if constexpr (kSorted) {
-            // the keys to shared memory, a 0 behind them: the owner of a round's key reads its next one, instead of moving all up
+            // the keys to shared memory, zeros behind each run: the owner of a round's key reads the next one, instead of moving all up
             unsigned* mine_at = &sorted[warp][lane * kRoom];
-            if constexpr (PER % 4 == 0) {
+            unsigned run[kRuns];
+            uint32_t from[kRuns];
 #pragma unroll
-                for (int i = 0; i < PER; i += 4) *reinterpret_cast<uint4*>(mine_at + i) = make_uint4(key[i], key[(i + 1) % PER], key[(i + 2) % PER], key[(i + 3) % PER]);
-            } else {
+            for (int r = 0; r < kRuns; ++r) {
+                unsigned* at = mine_at + r * (kRun + 4);
+                if constexpr (kRun % 4 == 0) {
 #pragma unroll
-                for (int i = 0; i < PER; ++i) mine_at[i] = key[i];
+                    for (int i = 0; i < kRun; i += 4)
+                        *reinterpret_cast<uint4*>(at + i) = make_uint4(key[r * kRun + i], key[r * kRun + (i + 1) % kRun], key[r * kRun + (i + 2) % kRun], key[r * kRun + (i + 3) % kRun]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kRun; ++i) at[i] = key[i];
+                }
+                run[r] = key[r * kRun];
+                from[r] = uint32_t(__cvta_generic_to_shared(at));
+                head = max(head, run[r]);
             }
-            uint32_t from = uint32_t(__cvta_generic_to_shared(mine_at)), to = uint32_t(__cvta_generic_to_shared(winners[warp]));
-            for (int s = 0; s <= p.k; ++s, to += 4) {
+            uint32_t to = uint32_t(__cvta_generic_to_shared(winners[warp]));
+            for (int s = 0; s < p.k + 2; ++s, to += 4) {
                 const unsigned top = __reduce_max_sync(dq::kFull, head);
-                asm volatile("{\n\t.reg .pred q;\n\t"
-                             "setp.eq.u32 q, %0, %2;\n\t"
-                             "@q st.shared.u32 [%3], %2;\n\t"
-                             "@q add.u32 %1, %1, 4;\n\t"
-                             "@q ld.shared.u32 %0, [%1];\n\t}"
-                             : "+r"(head), "+r"(from)
-                             : "r"(top), "r"(to)
-                             : "memory");
+                head = 0;
+#pragma unroll
+                for (int r = 0; r < kRuns; ++r) {
+                    asm volatile("{\n\t.reg .pred q;\n\t"
+                                 "setp.eq.u32 q, %0, %2;\n\t"
+                                 "@q st.shared.u32 [%3], %2;\n\t"
+                                 "@q add.u32 %1, %1, 4;\n\t"
+                                 "@q ld.shared.u32 %0, [%1];\n\t}"
+                                 : "+r"(run[r]), "+r"(from[r])
+                                 : "r"(top), "r"(to)
+                                 : "memory");
+                    head = max(head, run[r]);
+                }
             }
         } else {
 #pragma unroll
             for (int i = 1; i < PER; ++i) head = max(head, key[i]);
-            for (int s = 0; s <= p.k; ++s) {
+            for (int s = 0; s < p.k + 2; ++s) {
                 const unsigned top = __reduce_max_sync(dq::kFull, head);
                 if (head == top) {
                     winners[warp][s] = top;
@@ -439,12 +464,38 @@ __global__ void __launch_bounds__(128, PER <= 8 ? 8 : PER == 16 ? 4 : 2) k_moe_r
             }
         }
         __syncwarp();
-        const unsigned won = winners[warp][lane], after = winners[warp][lane + 1];   // of lane s < k: the s-th key, and the next
+        const unsigned won = winners[warp][lane], after = winners[warp][lane + 1];   // of lane s <= k: the s-th key, and the next
+        const unsigned last = winners[warp][p.k - 1], beyond = winners[warp][p.k + 1];
         __syncwarp();
-        if (!kExact) unsure |= lane < p.k && after != 0u && (won >> kPlace) - (after >> kPlace) <= near;
-        if (ORDER == kByLogit && F32) unsure |= lane < p.k && (won >> kPlace & ((1u << kSteps) - 1)) <= 4u;
         const int owner = 31 - int(won >> Log2<PER>::v & 31u);
         int mine = (owner >> log_p) * p.gs + (owner & (p.P - 1)) * p.q + (PER - 1 - int(won & (PER - 1)));
+        if constexpr (!kExact) {
+            bool close = lane < p.k && after != 0u && (won >> kPlace) - (after >> kPlace) <= near;
+            if (ORDER == kByLogit) unsure |= lane < p.k && (won >> kPlace & ((1u << kSteps) - 1)) <= 4u;
+            if (__any_sync(dq::kFull, close)) {
+                // neighbours too close for the keys: the k + 1 first anew by their scores in 64 bits, one a lane, where the one
+                // behind them cannot be among the k (and softmax has its sum in 32 bits: not here)
+                const bool apart = ORDER != kSoftmax && p.k < 32 && (beyond == 0u || (last >> kPlace) - (beyond >> kPlace) > near);
+                if (apart && !__any_sync(dq::kFull, unsure)) {
+                    const bool one = lane < p.k || (lane == p.k && won != 0u);
+                    double c = -INFINITY;
+                    if (one) {
+                        c = logit_at<F32>(row, mine);
+                        if (ORDER == kSigmoid) c = 1.0 / (1.0 + exp(-c)) + (p.bias ? double(p.bias[mine]) : 0.0);
+                    }
+                    int before = 0;
+                    for (int j = 0; j <= p.k; ++j) {
+                        const double oc = __shfl_sync(dq::kFull, c, j);
+                        const int oe = __shfl_sync(dq::kFull, mine, j);
+                        before += oc > c || (oc == c && oe < mine);
+                    }
+                    if (one) winners[warp][before] = unsigned(mine);
+                    __syncwarp();
+                    mine = int(winners[warp][lane]);
+                    __syncwarp();
+                } else unsure = true;
+            }
+        }
         bool nan = false;
         if (__any_sync(dq::kFull, unsure)) {
             const Again o = choose_again<PER, F32>(row, cnt, base, ORDER, top2, !(sigmoid || p.renorm), p);
@@ -530,7 +581,7 @@ std::string route_tokens(const void* logits, bool f32, long long ld, const berth
     // four logits per access where every lane's experts begin on a multiple of four of an aligned row
     const int size = f32 ? 4 : 2;
     const bool wide = p.gs % 4 == 0 && p.q % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) | uintptr_t(T > 1 ? ld * size : 0)) % (4 * size) == 0;
-    const int blocks = std::min((T + 3) / 4, 148 * 8);
+    const int blocks = std::min((T + 3) / 4, 148 * min_blocks(per));
     auto go = [&](auto launcher) { launcher(f32, by_logit ? kByLogit : score, score == kSigmoid, p, top2, wide, blocks, st); };
     switch (per) {
         case 1: go(launch<1>); break;
