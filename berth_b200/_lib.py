@@ -85,6 +85,7 @@ SIGNATURES = {
     "berth_exl3_last_error": (C.c_char_p, []),
     "berth_exl3_last_launch": (C.c_char_p, []),
     "berth_device_cc": (_i, [_i]),
+    "berth_device_current": (_i, []),
     "berth_device_sms": (_i, [_i]),
     "berth_device_status": (_i, [_i]),
     "berth_exl3_decode_rate": (_i, [_i] * 5 + [C.POINTER(C.c_double)] * 2),
@@ -163,6 +164,25 @@ def build(verbose: bool = False) -> str:
     out = None if verbose else subprocess.DEVNULL
     subprocess.run(["make", "-C", CSRC, "-j8"], check=True, stdout=out)
     return SO_PATH
+
+
+_bind = None
+
+
+def bind():
+    """The compiled callers of the operators that read torch tensors (csrc/bind.c).  Raises if they have not been built."""
+    global _bind
+    if _bind is None:
+        lib()
+        import torch
+        from .kernels import Error
+        try:
+            from . import _bind as module
+        except ImportError as exc:
+            raise RuntimeError(f"berth_b200/_bind.so cannot be loaded ({exc}): build it with `make -C {CSRC}`") from exc
+        module.init(Error, torch)
+        _bind = module
+    return _bind
 
 
 def lib() -> C.CDLL:

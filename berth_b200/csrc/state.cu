@@ -116,6 +116,11 @@ extern "C" int berth_device_cc(int device)
     try { return device_info(device).cc; } catch (const std::exception&) { cudaGetLastError(); return -1; }
 }
 
+extern "C" int berth_device_current(void)
+{
+    try { return current_device(); } catch (const std::exception&) { cudaGetLastError(); return -1; }
+}
+
 extern "C" int berth_device_status(int device)
 {
     try { return berth::read_gemv_status(device) | berth::read_static_status(device); } catch (const std::exception&) { cudaGetLastError(); return -1; }

@@ -10,7 +10,6 @@ the library raises :class:`Error` with the library's message, as ``Error::Launch
 from __future__ import annotations
 
 import enum
-from sys import modules as _modules
 
 from . import _lib
 
@@ -48,41 +47,6 @@ def _stream(stream):
 
 def _s(b) -> str:
     return (b or b"").decode("utf-8", "replace")
-
-
-def _device_of(what: str, *tensors) -> None:
-    """For the callers that take shapes and strides from torch tensors: refuses tensors that are not all on the current CUDA
-    device, which is the one the library launches on."""
-    device = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise Error(f"{what}: the tensors are on several devices")
-    if device < 0:
-        raise Error(f"{what}: every tensor must be on the CUDA device")
-    if device != torch_module().cuda.current_device():
-        raise Error(f"{what}: the tensors are on device {device}, the current device is {torch_module().cuda.current_device()}")
-
-
-def torch_module():
-    """torch, which a caller that holds tensors has imported (this module itself does without)."""
-    torch = _modules.get("torch")
-    if torch is None:
-        raise Error("torch tensors are expected")
-    return torch
-
-
-def _flat(what: str, name: str, t, dtype, *shape) -> None:
-    if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
-        raise Error(f"{what}: {name} must be a contiguous {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-
-
-def _is_f32(what: str, t) -> int:
-    torch = torch_module()
-    if t.dtype is torch.float32:
-        return 1
-    if t.dtype is torch.float16:
-        return 0
-    raise Error(f"{what}: fp16 or fp32 is expected, got {t.dtype}")
 
 
 def last_launch() -> str:
@@ -371,43 +335,8 @@ class ops:
         fp16 or fp32; the outputs may be the inputs themselves.  ``positions`` int32 ``[tokens]``; ``inv_freq`` float64, one entry per
         pair (``rope_frequencies``), so ``2 * len(inv_freq)`` elements of a head turn: neighbours when ``interleaved``, else i and
         i + len(inv_freq).  The formulas are at ``berth_ops_rope`` in include/berth_b200.h."""
-        torch = torch_module()
-        _device_of("rope", q, k, positions, inv_freq, q_out, k_out, q_norm, k_norm)
-        if q.dim() != 3:
-            raise Error(f"rope: q must be [tokens][heads][head_dim], got {tuple(q.shape)}")
-        (tokens, heads, dim), dtype = q.shape, q.dtype
-        f32 = _is_f32("rope", q)
-        if positions.dtype is not torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous():
-            raise Error("rope: positions must be a contiguous int32 tensor with one entry per token")
-        if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-            raise Error("rope: inv_freq must be a contiguous float64 tensor of one dimension")
-        if q_out.dtype is not dtype or q_out.shape != q.shape:
-            raise Error("rope: q_out must have the type and shape of q")
-        xt, xh, xe = q.stride()
-        yt, yh, ye = q_out.stride()
-        if (xe != 1 or ye != 1) and dim > 1:
-            raise Error("rope: the elements of a head must be contiguous")
-        if q_norm is not None and (q_norm.dtype is not torch.bfloat16 or q_norm.shape != (dim,) or not q_norm.is_contiguous()):
-            _flat("rope", "q_norm", q_norm, torch.bfloat16, dim)
-        rows_q = _lib.RopeRows(q.data_ptr(), q_out.data_ptr(), None if q_norm is None else q_norm.data_ptr(), xt, xh, yt, yh, heads)
-        rows_k = None
-        if k is not None and k_out is not None:
-            k_heads = k.shape[1] if k.dim() == 3 else -1
-            if k.dtype is not dtype or k.shape != (tokens, k_heads, dim) or k_out.dtype is not dtype or k_out.shape != k.shape:
-                raise Error("rope: k must share type, tokens and head_dim with q, and k_out have the type and shape of k")
-            xt, xh, xe = k.stride()
-            yt, yh, ye = k_out.stride()
-            if (xe != 1 or ye != 1) and dim > 1:
-                raise Error("rope: the elements of a head must be contiguous")
-            if k_norm is not None and (k_norm.dtype is not torch.bfloat16 or k_norm.shape != (dim,) or not k_norm.is_contiguous()):
-                _flat("rope", "k_norm", k_norm, torch.bfloat16, dim)
-            rows_k = _lib.RopeRows(k.data_ptr(), k_out.data_ptr(), None if k_norm is None else k_norm.data_ptr(), xt, xh, yt, yh, k_heads)
-        elif k is not None or k_out is not None or k_norm is not None:
-            raise Error("rope: k, k_out and k_norm go together")
-        rc = _lib.lib().berth_ops_rope(rows_q, rows_k, positions.data_ptr(), inv_freq.data_ptr(), tokens, dim, 2 * inv_freq.shape[0], interleaved,
-                                       attention_factor, norm_epsilon, norm_bias, f32, _stream(stream))
-        if rc != 0:
-            raise Error(ops.last_error() or f"rope launch failed ({rc})")
+        (_lib._bind or _lib.bind()).rope(q, k, positions, inv_freq, q_out, k_out, interleaved, attention_factor, q_norm, k_norm, norm_epsilon, norm_bias,
+                                         _stream(stream))
 
     ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
 
@@ -432,31 +361,4 @@ class ops:
         stride; ``vocab`` defaults to all columns): ``logprob`` fp32 and ``rank`` int32 ``[rows]`` of ``tokens`` (int32 ``[rows]``),
         ``entropy`` fp32 ``[rows]``, ``top_idx`` int32 and ``top_logprob`` fp32 ``[rows][n]``, n <= 32, the best alternatives.  Any output
         may be ``None``.  Masks, ties and padding tokens: ``berth_ops_logprobs`` in include/berth_b200.h."""
-        torch = torch_module()
-        _device_of("logprobs", logits, tokens, logprob, rank, entropy, top_idx, top_logprob)
-        if logits.dim() != 2:
-            raise Error(f"logprobs: logits must be [rows][vocab], got {tuple(logits.shape)}")
-        (rows, cols), (row_stride, elem) = logits.shape, logits.stride()
-        if elem != 1 and cols > 1:
-            raise Error("logprobs: the rows of logits must be contiguous")
-        if vocab is None:
-            vocab = cols
-        elif vocab > cols:
-            raise Error(f"logprobs: vocab {vocab} exceeds the {cols} columns of logits")
-        f32 = _is_f32("logprobs", logits)
-        i32, real = torch.int32, torch.float32
-        per_row = (rows,)
-        for name, t, dtype in (("tokens", tokens, i32), ("logprob", logprob, real), ("rank", rank, i32), ("entropy", entropy, real)):
-            if t is not None and (t.dtype is not dtype or t.shape != per_row or not t.is_contiguous()):
-                _flat("logprobs", name, t, dtype, rows)
-        n = 0
-        if top_idx is not None and top_logprob is not None:
-            n = top_idx.shape[-1]
-            _flat("logprobs", "top_idx", top_idx, i32, rows, n)
-            _flat("logprobs", "top_logprob", top_logprob, real, rows, n)
-        elif top_idx is not None or top_logprob is not None:
-            raise Error("logprobs: top_idx and top_logprob go together")
-        rc = _lib.lib().berth_ops_logprobs(logits.data_ptr(), f32, row_stride, _ptr(tokens), inv_temp, _ptr(logprob), _ptr(rank), _ptr(entropy),
-                                           _ptr(top_idx) if n else None, _ptr(top_logprob) if n else None, n, rows, vocab, _stream(stream))
-        if rc != 0:
-            raise Error(ops.last_error() or f"logprobs launch failed ({rc})")
+        (_lib._bind or _lib.bind()).logprobs(logits, tokens, logprob, rank, entropy, top_idx, top_logprob, vocab, inv_temp, _stream(stream))

@@ -14,7 +14,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .kernels import Error, _device_of, _flat, _is_f32, _ptr, _s, _stream
+from .kernels import Error, _ptr, _s, _stream
 
 _PTR_FIELDS = [n for n, _ in _lib.MoeWeights._fields_[7:]]
 
@@ -57,19 +57,10 @@ def route(logits, selection_bias, topk_idx, topk_w, top_k: int, score: str = "so
     """The experts of every token from its router logits (fp16 or fp32 ``[T][n_experts]``, rows of any stride): ``topk_idx`` int32 and
     ``topk_w`` fp32 ``[T][top_k]``.  ``selection_bias`` (fp32 ``[n_experts]`` or ``None``) takes part in the choice only.  The formulas
     and what happens to masked and NaN logits are at ``berth_moe_routing`` in include/berth_b200.h."""
-    _device_of("moe route", logits, selection_bias, topk_idx, topk_w)
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise Error("moe route: logits must be [T][n_experts] with contiguous rows")
-    T, E = logits.shape
-    f32 = _is_f32("moe route", logits)
-    _flat("moe route", "selection_bias", selection_bias, torch.float32, E)
-    _flat("moe route", "topk_idx", topk_idx, torch.int32, T, top_k)
-    _flat("moe route", "topk_w", topk_w, torch.float32, T, top_k)
-    sc, gs = _choice(score, group_score)
-    rc = _lib.lib().berth_moe_route(logits.data_ptr(), f32, logits.stride(0), _ptr(selection_bias), topk_idx.data_ptr(), topk_w.data_ptr(), T, E,
-                                    top_k, sc, n_group, topk_group, gs, renormalize, scale, _stream(stream))
-    if rc != 0:
-        raise Error(last_error() or f"moe route launch failed ({rc})")
+    sc, gs = SCORES.get(score), GROUP_SCORES.get(group_score)
+    if sc is None or gs is None:
+        _choice(score, group_score)
+    (_lib._bind or _lib.bind()).route(logits, selection_bias, topk_idx, topk_w, top_k, sc, n_group, topk_group, gs, renormalize, scale, _stream(stream))
 
 
 class Routing:

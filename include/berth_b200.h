@@ -92,6 +92,8 @@ int berth_exl3_weights_streamed(int on);
 /* Device queries of crates/berth-kernels/csrc/internal.h:11-13 (class 1..5 as the fork's CC_*
  * enumeration orders them: old, Ampere, Ada, Hopper, Blackwell; SM count). -1 on error. */
 int berth_device_cc(int device);
+/* The calling thread's current device, on which every entry point here launches (no counterpart in berth). -1 on error. */
+int berth_device_current(void);
 int berth_device_sms(int device);
 /* Reads and clears the status words of the kernels on `device`: the library's workspace and the
  * fixed scratch of berth_exl3_linear_static_scratch, OR-ed together (this call synchronises the
