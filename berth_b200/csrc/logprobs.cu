@@ -264,7 +264,6 @@ struct Shared {
     float m[kMaxCluster * WARPS], z[kMaxCluster * WARPS], t[kMaxCluster * WARPS];   // first CTA: the parts of the cluster's warps
     int before[kMaxCluster * WARPS];
     alignas(16) float reach[kMaxCluster * WARPS > 32 ? kMaxCluster * WARPS : 32];   // what logits of every warp of the cluster reach
-    alignas(16) float ranked[WARPS][32];
     int cand[WARPS][32];
     unsigned n_own, n_keys, flooded;
     float row_m, row_lnz;
@@ -281,7 +280,6 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
     using E = typename std::conditional<F32, float, __half>::type;
     constexpr int U = kUnroll, kThreads = WARPS * 32;
     __shared__ Shared<WARPS> sh;
-    pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int cta, ctas;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
@@ -461,16 +459,13 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
         if (warps >= 32)
             for (int i = lane; i < warps; i += 32) x = fmaxf(x, sh.reach[i]);
         else if (lane < warps << k_shift) x = sh.reach[lane];
-        sh.ranked[warp][lane] = x;
-        __syncwarp();
-        int place = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 o = reinterpret_cast<const float4*>(sh.ranked[warp])[i];
-            place += (o.x > x || (o.x == x && 4 * i < lane)) + (o.y > x || (o.y == x && 4 * i + 1 < lane)) + (o.z > x || (o.z == x && 4 * i + 2 < lane)) +
-                     (o.w > x || (o.w == x && 4 * i + 3 < lane));
+        float tau = 0.f;
+        const bool down = p.top_n <= 16;   // from the nearer end
+        const float gone = down ? -INFINITY : INFINITY;
+        for (int i = down ? p.top_n : 33 - p.top_n; i > 0; --i) {
+            tau = down ? redux_max(x) : redux_min(x);
+            if (lane == __ffs(__ballot_sync(dq::kFull, x == tau)) - 1) x = gone;
         }
-        const float tau = __shfl_sync(dq::kFull, x, __ffs(__ballot_sync(dq::kFull, place == p.top_n - 1)) - 1);
 
         const int room = kKeys / ctas;
         const uint32_t keys0 = peer_addr(&sh.keys[cta * room], 0);
@@ -532,6 +527,9 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
             sync_all();
         }
     }
+    // the next kernel on the stream comes now: at the start, its blocks took places that this one's later blocks wait for
+    // (77 rows of 100003 fp32: 13.1 -> 10.2 us a call, 421 of 32003: 18.8 -> 16.1)
+    pdl_trigger();
     if (cta != 0) return;
 
     // ---- the first CTA writes the row's answers: its last warp joins the parts, and all of them order the keys
