@@ -89,7 +89,7 @@ __device__ __forceinline__ void norm8(float* x, const void* w, int at, float rin
     }
 }
 
-constexpr int kThreads = 256, kTable = 2048;   // cos / sin pairs a block holds
+constexpr int kThreads = 128, kTable = 2048;   // cos / sin pairs a block holds
 
 // A block takes p.tile tokens: it fills a table of their cos and sin (one thread per pair and token, 64-bit angles), then groups of
 // p.lanes lanes walk the heads, each lane sixteen elements of a head.  A group stays with its token, so a lane's eight pairs of cos
@@ -194,10 +194,15 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
     }
 }
 
+// Bound: HBM.  8192 tokens of 40 heads of 128 fp16: 30.2 us (5.6 TB/s; with 256 threads a block 31.8), normalised 35.4; 421 tokens of 28
+// heads of 256, a quarter turned, normalised: 5.5 us.
+
 // The same for any part, alignment and stride: a lane holds sixteen consecutive elements and finds the other element of a pair
-// in shared memory (pitch 17, so that lanes 16 elements apart meet different banks).
+// in shared memory (pitch 17, so that lanes 16 elements apart meet different banks).  Its cos, signed sin and the places of the other
+// elements stay in registers.  Bound: the shared-memory traffic of 8 bytes an element.  4096 tokens of 40 heads of 128 fp16, 88 turned:
+// 27.1 us (k_rope with all 128 turned: 16.7); registers for 4 blocks an SM instead of 5: 31.5 us.
 template <typename T, bool NORM>
-__global__ void __launch_bounds__(kThreads) k_rope_any(const RopeParams p, bool wide)
+__global__ void __launch_bounds__(kThreads, 5) k_rope_any(const RopeParams p, bool wide)
 {
     __shared__ float2 table[kTable + kTable / 16 + kThreads];   // (pitch: half_rot + half_rot / 16 + 1, at most kThreads tokens)
     __shared__ float stage[kThreads * 17];
@@ -213,7 +218,20 @@ __global__ void __launch_bounds__(kThreads) k_rope_any(const RopeParams p, bool 
     }
     __syncthreads();
     float* mine = stage + (tid - lane) * 17;   // the group's head
-    const float2* cs = table + slot * pitch;
+    // out = v * cos + other * sin, with the sign of the pair's side; the group stays with its token
+    float2 cs[16];
+    int other_at[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int e = e0 + j;
+        const bool second = p.interleaved ? e & 1 : e >= p.half_rot;
+        const int k = p.interleaved ? e / 2 : second ? e - p.half_rot : e, o = second ? e - p.half_rot : e + p.half_rot;
+        if (e < p.rot) {
+            cs[j] = table[slot * pitch + k + k / 16];
+            if (!second) cs[j].y = -cs[j].y;
+            other_at[j] = o + o / 16;
+        }
+    }
     const int step = groups_per_token * gridDim.y, h0 = blockIdx.y * groups_per_token;
     for (int base = h0; base < heads; base += step) {
         const int h = base + group % groups_per_token;
@@ -240,36 +258,31 @@ __global__ void __launch_bounds__(kThreads) k_rope_any(const RopeParams p, bool 
             for (int off = p.lanes / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(dq::kFull, s, off);
             if (live && r.norm) {
                 const float rinv = rsqrtf(s / float(p.dim) + p.eps);
+                if (wide && e0 + 16 <= p.dim) {
+                    norm8(v, r.norm, e0, rinv, p.bias);
+                    norm8(v + 8, r.norm, e0 + 8, rinv, p.bias);
+                } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (e0 + j < p.dim) v[j] = v[j] * rinv * (bf16_at(r.norm, e0 + j) + p.bias);
+                    for (int j = 0; j < 16; ++j)
+                        if (e0 + j < p.dim) v[j] = v[j] * rinv * (bf16_at(r.norm, e0 + j) + p.bias);
+                }
             }
         }
         if (p.interleaved) {
 #pragma unroll
             for (int j = 0; j < 16; j += 2)
                 if (e0 + j < p.rot) {
-                    const int k = (e0 + j) / 2;
-                    const float2 c = cs[k + k / 16];
                     const float a = v[j], b = v[j + 1];
-                    v[j] = a * c.x - b * c.y;
-                    v[j + 1] = b * c.x + a * c.y;
+                    v[j] = a * cs[j].x + b * cs[j].y;
+                    v[j + 1] = b * cs[j + 1].x + a * cs[j + 1].y;
                 }
         } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j) mine[lane * 17 + j] = v[j];
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int e = e0 + j;
-                if (e < p.rot) {
-                    const bool second = e >= p.half_rot;
-                    const int k = second ? e - p.half_rot : e, o = second ? k : e + p.half_rot;
-                    const float2 c = cs[k + k / 16];
-                    const float other = mine[o + o / 16];
-                    v[j] = second ? v[j] * c.x + other * c.y : v[j] * c.x - other * c.y;
-                }
-            }
+            for (int j = 0; j < 16; ++j)
+                if (e0 + j < p.rot) v[j] = v[j] * cs[j].x + mine[other_at[j]] * cs[j].y;
             __syncwarp();
         }
         if (!live) continue;
@@ -331,7 +344,7 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     // few tokens: their heads over several blocks
     const int blocks_x = (p.tokens + p.tile - 1) / p.tile;
     int blocks_y = 1;
-    while (blocks_x * blocks_y < 148 && blocks_y * groups / p.tile < heads) ++blocks_y;
+    while (blocks_x * blocks_y < 148 * 4 && blocks_y * groups / p.tile < heads) ++blocks_y;
     const dim3 grid(blocks_x, blocks_y);
     std::string name;
     auto go = [&](auto kern, const char* what, auto... more) {
