@@ -150,20 +150,6 @@ __device__ __forceinline__ float redux_min(float v) { float r; asm("redux.sync.m
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
-// One warp per token; lane = P lanes per group, q consecutive experts each.
-//
-// The choice is made in 32 bits first and repeated in 64 (choose64) where that cannot tell.  An expert's key is its choice score in
-// fixed point with its place, (31 - lane, PER - 1 - i), in the lowest bits: keys differ, the larger key is the larger score or of
-// equal ones the lower expert, and a round of the choice is one redux over the lanes' heads.  A lane keeps its keys sorted.
-//   scores + bias: 2^QB steps over [least bias, 1 + largest bias];  fp32 logits by themselves: over the 32 below the row's largest;
-//   fp16 logits by themselves: the order of their bits, which have room for the place: exact.
-// Where two neighbours in the order (the first expert not chosen among them) lie closer than both scores' errors and the steps, the
-// k + 1 first are ordered anew in 64 bits, one a lane; the whole choice is repeated where that may not be enough (a third one as
-// close, a softmax under a bias, the last group kept and the first one dropped as close) and for a row that has an infinite or NaN logit.
-// Errors of c = s + b in units of 2^-24: sigmoid, s (1 - s) (1.5 |l| + 4) for exp and 3 for sum and reciprocal, below 4.5 each;
-// softmax, s (2.5 |l - m| + 7) <= 9 each and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below 2 (28 + PER) for a pair; the sum
-// with the bias, and the bias less the least, half a step of at most the span each.
-// Bound: instructions (some 27 an expert of a lane).  16384 tokens of 256 experts, 8 groups: %%
 // A row whose choice 32 bits cannot tell, or with an infinite or NaN logit: its logits once more, the choice in 64 bits, and what a
 // softmax over the row needs.
 struct Again {
@@ -203,16 +189,77 @@ __device__ __forceinline__ unsigned ordered(float v)
 template <int PER> struct Log2 { static constexpr int v = 1 + Log2<PER / 2>::v; };
 template <> struct Log2<1> { static constexpr int v = 0; };
 
-// Blocks of an SM that the registers have to allow, and the grid fills once: eight keys a lane, 16384 tokens, 6: 16.0 us, 8: 17.3 us; two
+// The two largest of a1 >= a2 and b1 >= b2.
+__device__ __forceinline__ void best_two(unsigned& a1, unsigned& a2, unsigned b1, unsigned b2)
+{
+    a2 = max(min(a1, b1), max(a2, b2));
+    a1 = max(a1, b1);
+}
+// The largest key of a group below its second one, k2 (keys differ).
+template <int PER>
+__device__ __forceinline__ unsigned third_key(const unsigned (&key)[PER], unsigned k2, int lanes)
+{
+    unsigned k3 = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) k3 = max(k3, key[i] < k2 ? key[i] : 0u);
+    for (int off = 1; off < lanes; off <<= 1) k3 = max(k3, __shfl_xor_sync(dq::kFull, k3, off));
+    return k3;
+}
+// The choice score of expert e in 64 bits (not for softmax, which needs its sum).
+template <bool F32, int ORDER>
+__device__ __forceinline__ double score64(const void* row, int e, const RouteParams& p)
+{
+    const double v = logit_at<F32>(row, e);
+    return ORDER == kByLogit ? v : 1.0 / (1.0 + exp(-v)) + (p.bias ? double(p.bias[e]) : 0.0);
+}
+// Whether this lane's group is kept, by the scores of the groups' two best experts (keys k1, k2; two lanes of a group or more).
+template <bool F32, int ORDER, int LOG_PER>
+__device__ __noinline__ bool groups_again(const void* row, unsigned k1, unsigned k2, int log_p, bool top2, const RouteParams& p)
+{
+    const int lane = threadIdx.x & 31, g = lane >> log_p, member = lane & (p.P - 1);
+    double c = -INFINITY;
+    const unsigned key = member == 0 ? k1 : k2;
+    if (g < p.G && member < 2 && key != 0u) {   // (groups of one expert: no second key)
+        const int owner = 31 - int(key >> LOG_PER & 31u);
+        c = score64<F32, ORDER>(row, (owner >> log_p) * p.gs + (owner & (p.P - 1)) * p.q + ((1 << LOG_PER) - 1 - int(key & ((1u << LOG_PER) - 1))), p);
+    }
+    const double other = __shfl_xor_sync(dq::kFull, c, 1);
+    const double worth = __shfl_sync(dq::kFull, top2 ? c + other : fmax(c, other), lane & ~(p.P - 1));
+    int before = 0;
+    for (int j = 0; j < p.G; ++j) {
+        const double o = __shfl_sync(dq::kFull, worth, j << log_p);
+        before += o > worth || (o == worth && j < g);
+    }
+    return before < p.keep;
+}
+
+// Blocks of an SM that the registers have to allow, and the grid fills once: eight keys a lane, 16384 tokens, 6: 13.8 us, 8: 14.7 us; two
 // keys a lane (64 experts) 8: 7.7 us, 6: 10.3 us.
 constexpr int min_blocks(int per) { return per < 8 ? 8 : per == 8 ? 6 : per == 16 ? 4 : 2; }
 
+// One warp per token; lane = P lanes per group, q consecutive experts each.
+//
+// The choice is made in 32 bits first and repeated in 64 (choose64) where that cannot tell.  An expert's key is its choice score in
+// fixed point with its place, (31 - lane, PER - 1 - i), in the lowest bits: keys differ, the larger key is the larger score or of
+// equal ones the lower expert, and a round of the choice is one redux over the lanes' heads.  A lane keeps its keys sorted.
+//   scores + bias: 2^23 steps (2^22 with 32 experts a lane, 2^21 with 64) over [least bias, 1 + largest bias];
+//   fp32 logits by themselves: as many over the 32 below the row's largest;
+//   fp16 logits by themselves: the order of their bits, which have room for the place: exact.
+// Where two neighbours in the order (the first expert not chosen among them) lie closer than both scores' errors and the steps, the
+// k + 1 first are ordered anew in 64 bits, one a lane; so are the groups by their two best experts, where the last one kept and the
+// first one dropped lie as close.  The whole choice is repeated where that may not be enough (a third one as close, a softmax under
+// a bias) and for a row that has an infinite or NaN logit.
+// Errors of c = s + b in units of 2^-24: sigmoid, s (1 - s) (1.5 |l| + 4) for exp and 3 for sum and reciprocal, below 4.5 each;
+// softmax, s (2.5 |l - m| + 7) <= 9 each and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below 2 (28 + PER) for a pair; the sum
+// with the bias, and the bias less the least, half a step of at most the span each.
+// Bound: instructions, half of them on the half-rate integer pipe, and their latency: 16384 tokens of 256 experts, 8 groups, 8 chosen
+// 13.8 us (17.8 MB would be 2.7), of which 2.5 are a call's least; all of it in 64 bits 57 us.
 template <int PER, bool F32, int ORDER>
 __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteParams p, bool sigmoid, bool top2, bool wide)
 {
     constexpr int kPlace = 5 + Log2<PER>::v, kSteps = 32 - kPlace < 23 ? 32 - kPlace : 23;
     constexpr int kRun = PER < 8 ? PER : 8, kRuns = PER / kRun, kRoom = (kRun + 4) * kRuns;   // a lane's keys: sorted runs, zeros behind each
-    constexpr unsigned kMask = (1u << kPlace) - 1;
+    constexpr unsigned kMask = (1u << kPlace) - 1, kScore = (1u << kSteps) - 1;
     constexpr bool kSorted = PER <= 32, kExact = ORDER == kByLogit && !F32, kHeldBias = PER <= 16 && ORDER != kByLogit, kAhead = PER <= 16;
     constexpr float kLog2e = 1.44269504088896341f, kUnit = 1.f / (1 << 24), kMagic = 8388608.f;   // 2^23 + n: n in the low bits
     __shared__ __align__(16) unsigned sorted[4][kSorted ? 32 * kRoom : 4];   // every lane's keys
@@ -338,38 +385,6 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
                 if (i >= cnt) c[i] = -FLT_MAX;
         }
 
-        // ---- groups: rounds over the lanes' (their groups') scores
-        bool open = g < p.G;
-        if (groups) {
-            float b1 = c[0], b2 = -FLT_MAX;
-#pragma unroll
-            for (int i = 1; i < PER; ++i) {
-                b2 = fmaxf(b2, fminf(b1, c[i]));
-                b1 = fmaxf(b1, c[i]);
-            }
-            for (int off = 1; off < p.P; off <<= 1) {
-                const float o1 = __shfl_xor_sync(dq::kFull, b1, off), o2 = __shfl_xor_sync(dq::kFull, b2, off);
-                b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
-                b1 = fmaxf(b1, o1);
-            }
-            const float score = top2 ? b1 + b2 : b1;
-            unsigned gkey, top = 0;
-            if constexpr (kExact) gkey = ordered(score) & ~31u;
-            else if constexpr (ORDER == kByLogit) gkey = __float_as_uint(fmaxf(fmaf(score - m, scale, kMagic + float((1 << kSteps) - 3)), kMagic)) << 5;
-            else gkey = __float_as_uint(fmaf(score, 0.5f * scale, kMagic + 1.f)) << 5;
-            gkey = open ? gkey | (31u - g) : 0u;
-            open = false;
-            for (int s = 0; s < p.keep; ++s) {
-                top = __reduce_max_sync(dq::kFull, gkey);
-                if (gkey == top) {
-                    open = true;
-                    gkey = 0;
-                }
-            }
-            if (!kExact) unsure |= (top >> 5) - (__reduce_max_sync(dq::kFull, gkey) >> 5) <= near;
-            if (ORDER == kByLogit && F32) unsure |= (top >> 5 & ((1u << kSteps) - 1)) <= 4u;   // (below the 32 of the logits, the steps end)
-        }
-
         // ---- keys, largest first
         unsigned key[PER];
         const unsigned place = (31u - lane) << Log2<PER>::v;
@@ -388,10 +403,6 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
             for (int i = 0; i < PER; ++i)
                 if (i >= cnt) key[i] = 0;
         }
-        if (!open) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) key[i] = 0;
-        }
         if constexpr (kSorted && PER > 1) {
 #pragma unroll
             for (int r = 0; r < PER; r += kRun)
@@ -408,7 +419,48 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
                                 key[r + j] = lo;
                             }
         }
-        unsigned head = key[0];
+        // ---- groups: the two best keys of each, rounds over the groups' worth
+        bool open = true;
+        if (groups) {
+            unsigned k1 = key[0], k2 = 0;
+            if constexpr (kSorted) {
+                if constexpr (PER > 1) k2 = key[1];
+#pragma unroll
+                for (int r = kRun; r < PER; r += kRun) best_two(k1, k2, key[r], key[r + (kRun > 1)]);
+            } else {
+#pragma unroll
+                for (int i = 1; i < PER; ++i) best_two(k1, k2, key[i], 0u);
+            }
+            for (int off = 1; off < p.P; off <<= 1) best_two(k1, k2, __shfl_xor_sync(dq::kFull, k1, off), __shfl_xor_sync(dq::kFull, k2, off));
+            // all lanes of a group hold the same; a sum has room for its group (both hold what the exponent left, the same in all)
+            const unsigned worth = !top2 ? k1 : (((k1 >> kPlace) & kScore) + ((k2 >> kPlace) & kScore)) << 5 | (31u - g);
+            const int low_bits = top2 ? 5 : kPlace;
+            unsigned gkey = g < p.G ? worth : 0u, top = 0;
+            open = false;
+            for (int s = 0; s < p.keep; ++s) {
+                top = __reduce_max_sync(dq::kFull, gkey);
+                if (gkey == top) {
+                    open = true;
+                    gkey = 0;
+                }
+            }
+            const unsigned next_one = __reduce_max_sync(dq::kFull, gkey);
+            if (!kExact && (top >> low_bits) - (next_one >> low_bits) <= near * (top2 ? 2 : 1)) {
+                // too close for the keys: the groups anew by their two best experts' scores in 64 bits, one a lane, where no group has
+                // a third one that could be the second
+                unsigned k3 = 0;
+                if constexpr (ORDER != kSoftmax && kSorted) {
+                    k3 = third_key<PER>(key, k2, p.P);
+                }
+                const bool apart = ORDER != kSoftmax && kSorted && p.P > 1 && (g >= p.G || k3 == 0u || (k2 >> kPlace) - (k3 >> kPlace) > near) &&
+                                   (ORDER != kByLogit || g >= p.G || ((k2 >> kPlace) & kScore) > 4u);
+                if (__all_sync(dq::kFull, apart) && !__any_sync(dq::kFull, unsure)) open = groups_again<F32, ORDER, Log2<PER>::v>(row, k1, k2, log_p, top2, p);
+                else unsure = true;
+            }
+            if (ORDER == kByLogit && F32) unsure |= (top >> kPlace & kScore) <= 4u;   // (below the 32 of the logits, the steps end)
+        }
+
+        unsigned head = open ? key[0] : 0u;
         if constexpr (kSorted) {
             // the keys to shared memory, zeros behind each run: the owner of a round's key reads the next one, instead of moving all up
             unsigned* mine_at = &sorted[warp][lane * kRoom];
@@ -425,8 +477,8 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
 #pragma unroll
                     for (int i = 0; i < kRun; ++i) at[i] = key[i];
                 }
-                run[r] = key[r * kRun];
-                from[r] = uint32_t(__cvta_generic_to_shared(at));
+                run[r] = open ? key[r * kRun] : 0u;
+                from[r] = uint32_t(__cvta_generic_to_shared(open ? at : at + kRun));
                 head = max(head, run[r]);
             }
             uint32_t to = uint32_t(__cvta_generic_to_shared(winners[warp]));
@@ -448,7 +500,7 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
             }
         } else {
 #pragma unroll
-            for (int i = 1; i < PER; ++i) head = max(head, key[i]);
+            for (int i = 1; i < PER; ++i) head = max(head, open ? key[i] : 0u);
             for (int s = 0; s < p.k + 2; ++s) {
                 const unsigned top = __reduce_max_sync(dq::kFull, head);
                 if (head == top) {
@@ -471,18 +523,14 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
         int mine = (owner >> log_p) * p.gs + (owner & (p.P - 1)) * p.q + (PER - 1 - int(won & (PER - 1)));
         if constexpr (!kExact) {
             bool close = lane < p.k && after != 0u && (won >> kPlace) - (after >> kPlace) <= near;
-            if (ORDER == kByLogit) unsure |= lane < p.k && (won >> kPlace & ((1u << kSteps) - 1)) <= 4u;
+            if (ORDER == kByLogit) unsure |= lane < p.k && (won >> kPlace & kScore) <= 4u;
             if (__any_sync(dq::kFull, close)) {
                 // neighbours too close for the keys: the k + 1 first anew by their scores in 64 bits, one a lane, where the one
                 // behind them cannot be among the k (and softmax has its sum in 32 bits: not here)
                 const bool apart = ORDER != kSoftmax && p.k < 32 && (beyond == 0u || (last >> kPlace) - (beyond >> kPlace) > near);
                 if (apart && !__any_sync(dq::kFull, unsure)) {
                     const bool one = lane < p.k || (lane == p.k && won != 0u);
-                    double c = -INFINITY;
-                    if (one) {
-                        c = logit_at<F32>(row, mine);
-                        if (ORDER == kSigmoid) c = 1.0 / (1.0 + exp(-c)) + (p.bias ? double(p.bias[mine]) : 0.0);
-                    }
+                    const double c = one ? score64<F32, ORDER>(row, mine, p) : -INFINITY;
                     int before = 0;
                     for (int j = 0; j <= p.k; ++j) {
                         const double oc = __shfl_sync(dq::kFull, c, j);
