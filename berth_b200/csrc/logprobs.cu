@@ -488,7 +488,8 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
                             const int i = sh.cand[warp][c] + (step * U + (lane & 3)) * stride;
                             if (i >= nvec) continue;
                             V w;
-                            w.load(vecs + i);
+                            if (steps <= 2) w.set(ring[((step & 1) * U + (lane & 3)) * kThreads + sh.cand[warp][c] - cta * kThreads]);   // still there
+                            else w.load(vecs + i);
                             if (w.max_with(-INFINITY) >= tau) {
 #pragma unroll
                                 for (int e = 0; e < V::N; ++e)
