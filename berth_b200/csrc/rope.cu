@@ -346,10 +346,10 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     int blocks_y = 1;
     while (blocks_x * blocks_y < 148 * 4 && blocks_y * groups / p.tile < heads) ++blocks_y;
     const dim3 grid(blocks_x, blocks_y);
-    std::string name;
+    const char* name = "";
     auto go = [&](auto kern, const char* what, auto... more) {
         launch_pdl(kern, grid, dim3(kThreads), 0, st, "rope launch", p, more...);
-        name = std::string(what) + "<" + (f32 ? "float" : "half") + (norm ? ",norm" : "") + ">";
+        name = what;
     };
     auto typed = [&](auto zero) {
         using T = decltype(zero);
@@ -359,8 +359,8 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     };
     if (f32) typed(0.0f);
     else typed(__half{});
-    return name + " block=" + std::to_string(kThreads) + " grid=" + std::to_string(blocks_x) + "x" + std::to_string(blocks_y) + " tokens=" +
-           std::to_string(p.tile) + " lanes=" + std::to_string(p.lanes);
+    return describe("%s<%s%s> block=%d grid=%dx%d tokens=%d lanes=%d", name, f32 ? "float" : "half", norm ? ",norm" : "", kThreads, blocks_x, blocks_y, p.tile,
+                    p.lanes);
 }
 
 }  // namespace

@@ -640,8 +640,7 @@ std::string route_tokens(const void* logits, bool f32, long long ld, const berth
         case 32: go(launch<32>); break;
         default: go(launch<64>); break;   // up to 1024 experts: q <= 64
     }
-    return "k_moe_route<" + std::to_string(per) + "," + (f32 ? "float" : "half") + "," + (score == kSigmoid ? "sigmoid" : "softmax") + (by_logit ? "" : ",scores") + "> grid=" +
-           std::to_string(blocks);
+    return describe("k_moe_route<%d,%s,%s%s> grid=%d", per, f32 ? "float" : "half", score == kSigmoid ? "sigmoid" : "softmax", by_logit ? "" : ",scores", blocks);
 }
 
 }  // namespace berth
