@@ -375,7 +375,7 @@ extern "C" int berth_ops_rope(const berth_rope_rows* q, const berth_rope_rows* k
     CallState& st = ops_state();
     return guarded(st, [&] {
         if (!q || !positions || !inv_freq) throw std::runtime_error("rope: null pointer");
-        if (n_tokens < 1) throw std::runtime_error("rope: n_tokens must be positive");
+        if (n_tokens < 1 || n_tokens > (1 << 30)) throw std::runtime_error("rope: n_tokens must be positive and at most 2^30");
         if (head_dim < 2 || head_dim > 512) throw std::runtime_error("rope: head_dim must be in 2..=512");
         if (rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim) throw std::runtime_error("rope: rot_dim must be positive, even and at most head_dim");
         if (fp32 != 0 && fp32 != 1) throw std::runtime_error("rope: fp32 must be 0 or 1");

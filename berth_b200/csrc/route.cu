@@ -655,7 +655,7 @@ extern "C" int berth_moe_route(const void* logits, int logits_fp32, int64_t row_
     return guarded(st, [&] {
         if (!logits || !topk_idx || !topk_w) throw std::runtime_error("moe route: null device pointer");
         if (logits_fp32 != 0 && logits_fp32 != 1) throw std::runtime_error("moe route: logits_fp32 must be 0 or 1");
-        if (T < 1) throw std::runtime_error("moe route: T must be positive");
+        if (T < 1 || T > (1 << 30)) throw std::runtime_error("moe route: T must be positive and at most 2^30");
         if (n_experts < 1 || n_experts > 1024) throw std::runtime_error("moe route: n_experts must be in 1..=1024");
         if (top_k < 1 || top_k > 32 || top_k > n_experts) throw std::runtime_error("moe route: top_k must be in 1..=32 and at most n_experts");
         if (row_stride < n_experts && T > 1) throw std::runtime_error("moe route: row_stride is smaller than n_experts");
