@@ -78,9 +78,9 @@ template <> struct Piece<float> {
         reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
     }
 };
-__device__ __forceinline__ void norm8(float* x, const void* w, int at, float rinv, float bias)
+__device__ __forceinline__ uint4 weights8(const void* w, int at) { return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + at); }
+__device__ __forceinline__ void norm8(float* x, const uint4& v, float rinv, float bias)
 {
-    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + at);
     const uint32_t h[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -126,19 +126,30 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
     };
     const int step = groups_per_token * gridDim.y;
     int h = blockIdx.y * groups_per_token + group % groups_per_token;
-    Piece<T> in[2];
-    const T* x = nullptr;
-    T* y = nullptr;
-    const void* norm = nullptr;
-    auto fetch = [&] {
+    // pieces of the next heads on their way while one is worked on: two heads of plain fp16 (8192 tokens of 40 heads of 128: 28.6 us,
+    // one: 30.2), one where there is a norm (35.1 us, two: 38.2) or fp32 (4096 tokens 32.6 us, two: 33.6)
+    constexpr int kAhead = NORM || sizeof(T) == 4 ? 1 : 2;
+    struct Head {
+        Piece<T> in[2];
+        T* y;
+        const void* norm;
+    } ahead[kAhead];
+    auto fetch = [&](Head& to, int h) {
         if (t < p.tokens && h < heads) {
-            rows_of(h, x, y, norm);
+            const T* x;
+            if constexpr (kAhead == 1) rows_of(h, x, to.y, to.norm);
+            else {   // (found again when it is worked on: four registers a head cost more than that)
+                T* y;
+                const void* norm;
+                rows_of(h, x, y, norm);
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (at[i] >= 0) in[i].load(x + at[i]);
+                if (at[i] >= 0) to.in[i].load(x + at[i]);
         }
     };
-    fetch();
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch(ahead[i], h + i * step);
     for (int i = tid; i < p.tile * p.half_rot; i += kThreads) {
         const int s = i / p.half_rot;
         if (t0 + s < p.tokens) table[i] = turn(p.positions[t0 + s], p.inv_freq[i - s * p.half_rot], p.factor);
@@ -149,21 +160,27 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
 #pragma unroll
         for (int i = 0; i < 8; ++i) if (8 * lane + i < p.half_rot) cs[i] = table[slot * p.half_rot + 8 * lane + i];
     }
-    // every lane of a warp walks alike, so that the norm's sums meet
-    for (int round = h; round - group % groups_per_token < heads; round += step) {
+    auto work = [&](Head& now) {
         float v[16];
-        T* to = y;
-        const void* w = norm;
         const bool live = t < p.tokens && h < heads;
+        T* to = nullptr;
+        const void* w = nullptr;
+        if constexpr (kAhead == 1) {
+            to = now.y;
+            w = now.norm;
+        } else if (live) {
+            const T* x;
+            rows_of(h, x, to, w);
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (live && at[i] >= 0) in[i].get(v + 8 * i);
+            if (live && at[i] >= 0) now.in[i].get(v + 8 * i);
             else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[8 * i + j] = 0.f;
             }
+        fetch(now, h + kAhead * step);
         h += step;
-        fetch();
         if constexpr (NORM) {
             float s = 0.f;
 #pragma unroll
@@ -173,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
                 const float rinv = rsqrtf(s / float(p.dim) + p.eps);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (at[i] >= 0) norm8(v + 8 * i, w, at[i], rinv, p.bias);
+                    if (at[i] >= 0) norm8(v + 8 * i, weights8(w, at[i]), rinv, p.bias);
             }
         }
         if (lane < turning) {
@@ -191,10 +208,17 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
             for (int i = 0; i < 2; ++i)
                 if (at[i] >= 0) Piece<T>::store(to + at[i], v + 8 * i);
         }
+    };
+    // every lane of a warp walks alike, so that the norm's sums meet
+    for (int base = blockIdx.y * groups_per_token; base < heads; base += kAhead * step) {
+        work(ahead[0]);
+        if constexpr (kAhead == 2) {
+            if (base + step < heads) work(ahead[1]);
+        }
     }
 }
 
-// Bound: HBM.  8192 tokens of 40 heads of 128 fp16: 30.2 us (5.6 TB/s; with 256 threads a block 31.8), normalised 35.4; 421 tokens of 28
+// Bound: HBM.  8192 tokens of 40 heads of 128 fp16: 28.6 us (5.9 TB/s; with 256 threads a block 31.8), normalised 33.8; 421 tokens of 28
 // heads of 256, a quarter turned, normalised: 5.5 us.
 
 // The same for any part, alignment and stride: a lane holds sixteen consecutive elements and finds the other element of a pair
@@ -259,8 +283,8 @@ __global__ void __launch_bounds__(kThreads, 5) k_rope_any(const RopeParams p, bo
             if (live && r.norm) {
                 const float rinv = rsqrtf(s / float(p.dim) + p.eps);
                 if (wide && e0 + 16 <= p.dim) {
-                    norm8(v, r.norm, e0, rinv, p.bias);
-                    norm8(v + 8, r.norm, e0 + 8, rinv, p.bias);
+                    norm8(v, weights8(r.norm, e0), rinv, p.bias);
+                    norm8(v + 8, weights8(r.norm, e0 + 8), rinv, p.bias);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -337,9 +361,10 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     p.lanes = 1;
     while (p.lanes < units) p.lanes *= 2;
     const int groups = kThreads / p.lanes;
-    // tokens of a block: until every group walks some four heads, as long as the grid has four blocks an SM
+    // tokens of a block: until every group walks some four heads, or eight where they are normalised (8192 tokens of 40 heads of 128:
+    // plain 28.6 us, with eight 28.8; normalised 33.8, with four 35.1), as long as the grid has four blocks an SM
     p.tile = 1;
-    while (p.tile < groups && heads * p.tile < 4 * groups && (p.tokens + 2 * p.tile - 1) / (2 * p.tile) >= 148 * 4 && 2 * p.tile * p.half_rot <= kTable)
+    while (p.tile < groups && heads * p.tile < (norm ? 8 : 4) * groups && (p.tokens + 2 * p.tile - 1) / (2 * p.tile) >= 148 * 4 && 2 * p.tile * p.half_rot <= kTable)
         p.tile *= 2;
     // few tokens: their heads over several blocks
     const int blocks_x = (p.tokens + p.tile - 1) / p.tile;
