@@ -263,7 +263,7 @@ struct Shared {
     unsigned long long lists[kKeys / 32][32];   // the warps' lists of the slow way; first CTA: the keys, one behind the other
     float m[kMaxCluster * WARPS], z[kMaxCluster * WARPS], t[kMaxCluster * WARPS];   // first CTA: the parts of the cluster's warps
     int before[kMaxCluster * WARPS];
-    alignas(16) float reach[kMaxCluster * WARPS > 32 ? kMaxCluster * WARPS : 32];   // what logits of every warp of the cluster reach
+    float reach[kMaxCluster * WARPS];           // what logits of every warp of the cluster reach
     int cand[WARPS][32];
     unsigned n_own, n_keys, flooded;
     float row_m, row_lnz;
@@ -427,11 +427,12 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
     const Part own = joined({Part{m, m > -INFINITY ? (z - 1.f) + z_low : z, t}}, p.scale2);
     if (RANK) before = __reduce_add_sync(dq::kFull, before);
     // one logit that a warp reaches, or with few warps its k largest threads: lane i the i-th
+    const bool many = p.top_n > (warps >= 16 ? 12 : warps == 8 ? 16 : 24);   // 64 groups, or 32 (see tau)
     int k_shift = 0;
     float reach = own.m;
-    if (p.top_n > 0 && warps < 32) {
+    if (p.top_n > 0 && warps < (many ? 64 : 32)) {
         k_shift = 1;
-        while (p.top_n > warps << k_shift) ++k_shift;
+        while (many ? warps << k_shift < 64 : warps << k_shift < p.top_n) ++k_shift;
         float rest = m, best = own.m;
         for (int i = 1; i < 1 << k_shift; ++i) {
             if (lane == __ffs(__ballot_sync(dq::kFull, rest == best)) - 1) rest = -INFINITY;
@@ -454,17 +455,33 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
 
     // ---- the candidates for the n best
     if (p.top_n > 0) {
-        // up to 32 different logits that the row reaches, of 32 groups of warps or of the warps' largest threads; tau: the n-th of them
-        float x = -INFINITY;
-        if (warps >= 32)
-            for (int i = lane; i < warps; i += 32) x = fmaxf(x, sh.reach[i]);
-        else if (lane < warps << k_shift) x = sh.reach[lane];
-        float tau = 0.f;
-        const bool down = p.top_n <= 16;   // from the nearer end
-        const float gone = down ? -INFINITY : INFINITY;
-        for (int i = down ? p.top_n : 33 - p.top_n; i > 0; --i) {
-            tau = down ? redux_max(x) : redux_min(x);
-            if (lane == __ffs(__ballot_sync(dq::kFull, x == tau)) - 1) x = gone;
+        // up to 32 or 64 different logits that the row reaches, of as many groups of warps or of the warps' largest threads; tau: the
+        // n-th of them, by rounds, or for a larger n close below it by bisection.  With 32 groups an n of 32 would let in all
+        // that exceeds the least of them, some 130 logits and now and then 300: 16 rows of 15390 fp32 11.8 us, now 6.5.
+        float x = -INFINITY, tau = 0.f;
+        const int values = warps << k_shift;
+        if (many) {
+            float y = -INFINITY;
+            for (int i = lane; i < values; i += 64) {
+                x = fmaxf(x, sh.reach[i]);
+                y = fmaxf(y, sh.reach[i + 32]);
+            }
+            const unsigned a = order_bits(x), b = order_bits(y);
+            unsigned lo = __reduce_min_sync(dq::kFull, min(a, b)), hi = __reduce_max_sync(dq::kFull, max(a, b));
+            for (int i = 0; i < 14 && lo < hi; ++i) {
+                const unsigned mid = lo + (hi - lo + 1) / 2;
+                if (__popc(__ballot_sync(dq::kFull, a >= mid)) + __popc(__ballot_sync(dq::kFull, b >= mid)) >= p.top_n) lo = mid;
+                else hi = mid - 1;
+            }
+            tau = key_value((unsigned long long) lo << 32);
+        } else {
+            for (int i = lane; i < values; i += 32) x = fmaxf(x, sh.reach[i]);
+            const bool down = p.top_n <= 16;   // from the nearer end
+            const float gone = down ? -INFINITY : INFINITY;
+            for (int i = down ? p.top_n : 33 - p.top_n; i > 0; --i) {
+                tau = down ? redux_max(x) : redux_min(x);
+                if (lane == __ffs(__ballot_sync(dq::kFull, x == tau)) - 1) x = gone;
+            }
         }
 
         const int room = kKeys / ctas;
@@ -622,23 +639,24 @@ void launch(const LogprobParams& p, int ctas, int warps, cudaStream_t st)
 }
 
 // How a row is split: CTAs of its cluster and warps of each.  Measured (us, rows x vocabulary, warps/CTAs):
-//   as many warps as run at once (4736), a power of two of them a row, none with less than 1 KB:
-//     32 x 248320 fp32 128 warps 13.6, 64 warps 16.2; 64 x 248320 fp16 64 warps 15.1, 128 warps 21.2; 1 x 5000 fp32 16 warps 4.8, 64 warps 5.0;
-//     at most 128: 16 x 248320 fp32 12.2, 256 warps 14.6;
+//   as many warps as run at once (4736, of which clusters fill nine tenths), a power of two of them a row, none with less than 1 KB:
+//     37 x 187037 fp16 64 warps 7.6, 128 warps 11.3 (4736 of them); 64 x 248320 fp16 64 warps 14.8, 128 warps 21.2; 1 x 5000 fp32 16 warps
+//     4.6, 64 warps 5.0; at most 128, above 16 rows 64: 16 x 248320 fp32 8/16 10.6, 16/16 14.6; 32 x 248320 fp32 8/8 12.8, 16/8 13.0;
 //   a second wave where the first would leave a quarter of the GPU idle and the parts are long:
-//     421 x 248320 fp16 16 warps 50.7, 8 warps 63.2; 150 x 250000 fp16 32 warps 27.1, 16 warps 34.9; not for 77 x 100003 fp32 (13.2 both);
-//   large clusters of small CTAs for few rows (1 x 32000 fp16 4/8 5.1, 16/2 6.2; 4 x 248320 fp32 8/16 7.6, 16/8 8.7), at most 8 CTAs
-//     above 16 rows (32 x 248320 fp32 16/8 13.6, 8/16 16.5), single CTAs above 148 rows of up to 16 warps (421 rows 16/1 50.7, 4/4 55.1).
+//     421 x 248320 fp16 16 warps 48, 8 warps 61; 150 x 250000 fp16 32 warps 26, 16 warps 35; 336 x 37714 fp32 8 warps 13.4, 16 warps 15.7;
+//   small CTAs in clusters of up to 8, of 16 for 128 warps: 1 x 32000 fp16 4/8 5.0, 16/2 6.2; 13 x 21619 fp32 8/8 6.3, 4/16 7.2;
+//     4 x 248320 fp32 8/16 7.4, 16/8 8.3; one CTA of 8 warps (1 x 2314 fp32 8/1 2.8, 4/2 3.2), and of 16 in a second wave (421 rows 16/1 48,
+//     4/4 53; in a first one 160 x 38881 fp32 4/4 13.6, 16/1 16.2).
 void row_split(int rows, long long row_bytes, int& ctas, int& warps)
 {
-    const long long at_once = 148 * 32;
+    const long long at_once = 148 * 32, limit = rows <= 16 ? 128 : 64;
     long long n = 4;
-    while (n < 128 && rows * n * 2 <= at_once && row_bytes >= n * 2 * 1024) n *= 2;
-    if (n < 128 && 4 * rows * n <= 3 * at_once && row_bytes > n * 16384) n *= 2;
-    if (n < 128 && rows > 148 && row_bytes > n * 49152) n *= 2;
-    const long long most = rows <= 16 ? 16 : rows <= 148 || n > 16 ? 8 : 1;
-    warps = int(std::min<long long>(16, std::max<long long>(4, n / most)));
-    ctas = int(n / warps);
+    while (n < limit && 10 * rows * n * 2 <= 9 * at_once && row_bytes >= n * 2 * 1024) n *= 2;
+    if (n < limit && 4 * rows * n <= 3 * at_once && row_bytes > n * 24576) n *= 2;
+    if (n < limit && rows > 148 && row_bytes > n * 49152) n *= 2;
+    const bool one_wave = 10 * rows * n <= 9 * at_once;
+    ctas = n <= 8 || (n == 16 && !one_wave) ? 1 : n == 16 ? 4 : n == 128 ? 16 : 8;
+    warps = int(n / ctas);
 }
 
 }  // namespace
