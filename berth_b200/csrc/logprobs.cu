@@ -270,6 +270,34 @@ struct Shared {
     int none;
 };
 
+// The slow way to a CTA's best: its vectors again, 32 sorted keys a warp, merged into sh.lists[0].
+template <bool F32, int WARPS>
+__device__ __noinline__ void sorted_lists(Shared<WARPS>& sh, const char* row, const uint4* vecs, int head, int nvec, int first, int stride, int single, float tau,
+                                          int n)
+{
+    using V = Vec<F32>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned long long list = 0;
+    offer_keys(list, single >= 0 ? order_key(value_at<F32>(row, single), single) : 0, n);
+    for (int base = first - lane; base < nvec; base += stride) {
+        const int i = base + lane;
+        V w;
+        w.clear();
+        if (i < nvec) w.load(vecs + i);
+#pragma unroll
+        for (int e = 0; e < V::N; ++e) offer_keys(list, i < nvec && !(w.at(e) < tau) ? order_key(w.at(e), head + i * V::N + e) : 0, n);
+    }
+    sh.lists[warp][lane] = list;
+    for (int w = WARPS / 2; w >= 1; w >>= 1) {
+        __syncthreads();
+        if (warp < w) {
+            list = merge_lists(list, sh.lists[warp + w][lane]);
+            sh.lists[warp][lane] = list;
+        }
+    }
+    __syncthreads();
+}
+
 // Vector i of the row belongs to thread i % kThreads of CTA (i / kThreads) % ctas, so that every warp sees all of the
 // vocabulary: a threshold taken from the warps' maxima then holds where the likely tokens lie close together.  The walk takes 4
 // vectors of a thread at a time, while those of the next step are on their way to shared memory.
@@ -468,7 +496,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
             }
             const unsigned a = order_bits(x), b = order_bits(y);
             unsigned lo = __reduce_min_sync(dq::kFull, min(a, b)), hi = __reduce_max_sync(dq::kFull, max(a, b));
-            for (int i = 0; i < 14 && lo < hi; ++i) {
+            for (int i = 0; i < 10 && lo < hi; ++i) {
                 const unsigned mid = lo + (hi - lo + 1) / 2;
                 if (__popc(__ballot_sync(dq::kFull, a >= mid)) + __popc(__ballot_sync(dq::kFull, b >= mid)) >= p.top_n) lo = mid;
                 else hi = mid - 1;
@@ -521,26 +549,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
             sync_all();
         }
         if (tau == -INFINITY || sh.flooded) {
-            // the CTA's vectors again, 32 sorted keys a warp
-            unsigned long long list = 0;
-            offer_keys(list, single >= 0 ? order_key(value_at<F32>(row, single), single) : 0, p.top_n);
-            for (int base = first - lane; base < nvec; base += stride) {
-                const int i = base + lane;
-                V w;
-                w.clear();
-                if (i < nvec) w.load(vecs + i);
-#pragma unroll
-                for (int e = 0; e < V::N; ++e) offer_keys(list, i < nvec && !(w.at(e) < tau) ? order_key(w.at(e), head + i * V::N + e) : 0, p.top_n);
-            }
-            sh.lists[warp][lane] = list;
-            for (int w = WARPS / 2; w >= 1; w >>= 1) {
-                __syncthreads();
-                if (warp < w) {
-                    list = merge_lists(list, sh.lists[warp + w][lane]);
-                    sh.lists[warp][lane] = list;
-                }
-            }
-            __syncthreads();
+            sorted_lists<F32, WARPS>(sh, row, vecs, head, nvec, first, stride, single, tau, p.top_n);
             for (int i = tid; i < room; i += kThreads) peer_store(keys0 + i * 8, i < p.top_n ? sh.lists[0][i] : 0ull);
             sync_all();
         }
