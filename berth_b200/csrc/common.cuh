@@ -73,6 +73,12 @@ __attribute__((format(printf, 1, 2))) inline std::string describe(const char* fo
     return text;
 }
 
+// Refuses a pointer that is not on a boundary of its elements (NULL is); what: "entry point: argument".
+inline void check_aligned(const void* p, size_t size, const char* what)
+{
+    if (reinterpret_cast<uintptr_t>(p) % size) throw std::runtime_error(std::string(what) + " is not aligned to its elements");
+}
+
 // Runs `fn`, turning any exception into rc -1 + message, clearing the sticky CUDA error the
 // way crates/berth-kernels/csrc/linear.cu:377-394 does.
 template <typename F>

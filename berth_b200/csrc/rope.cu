@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_rope_any(const RopeParams p, bo
 }
 
 // A copy of r with the strides that no element needs set to zero.
-berth_rope_rows checked_rows(const berth_rope_rows& r, const char* what, int tokens, int dim)
+berth_rope_rows checked_rows(const berth_rope_rows& r, const char* what, int tokens, int dim, int size)
 {
     auto fail = [&](const char* msg) { throw std::runtime_error(std::string("rope: ") + what + ": " + msg); };
     if (!r.x || !r.y) fail("null device pointer");
@@ -330,7 +330,16 @@ berth_rope_rows checked_rows(const berth_rope_rows& r, const char* what, int tok
     berth_rope_rows c = r;
     if (tokens == 1) c.x_token = c.y_token = 0;
     if (c.heads == 1) c.x_head = c.y_head = 0;
-    if ((tokens > 1 && std::llabs(c.y_token) < dim) || (c.heads > 1 && std::llabs(c.y_head) < dim)) fail("the heads of the output overlap");
+    check_aligned(r.x, size, (std::string("rope: ") + what).c_str());
+    check_aligned(r.y, size, (std::string("rope: output of ") + what).c_str());
+    check_aligned(r.norm, 2, (std::string("rope: norm of ") + what).c_str());
+    // an output's heads lie apart along the smaller of its strides, and all that walks the larger one
+    long long a = std::llabs(c.y_head), b = std::llabs(c.y_token), na = c.heads, nb = tokens;
+    if (nb > 1 && (na == 1 || b < a)) {
+        std::swap(a, b);
+        std::swap(na, nb);
+    }
+    if ((na > 1 && a < dim) || (nb > 1 && b < __int128(na - 1) * a + dim)) fail("the heads of the output overlap");
     if (c.x == c.y && (c.x_token != c.y_token || c.x_head != c.y_head)) fail("an output in place needs the strides of its input");
     return c;
 }
@@ -407,9 +416,11 @@ extern "C" int berth_ops_rope(const berth_rope_rows* q, const berth_rope_rows* k
         if (!std::isfinite(attention_factor)) throw std::runtime_error("rope: attention_factor must be finite");
         if ((q->norm || (k && k->norm)) && !(norm_epsilon >= 0.f && std::isfinite(norm_epsilon)))
             throw std::runtime_error("rope: norm_epsilon must be finite and not negative");
+        check_aligned(positions, 4, "rope: positions");
+        check_aligned(inv_freq, 8, "rope: inv_freq");
         RopeParams p{};
-        p.r[0] = checked_rows(*q, "q", n_tokens, head_dim);
-        if (k) p.r[1] = checked_rows(*k, "k", n_tokens, head_dim);
+        p.r[0] = checked_rows(*q, "q", n_tokens, head_dim, fp32 ? 4 : 2);
+        if (k) p.r[1] = checked_rows(*k, "k", n_tokens, head_dim, fp32 ? 4 : 2);
         p.positions = positions; p.inv_freq = inv_freq; p.tokens = n_tokens; p.dim = head_dim; p.rot = rot_dim; p.half_rot = rot_dim / 2;
         p.interleaved = interleaved != 0; p.factor = attention_factor; p.eps = norm_epsilon; p.bias = norm_bias;
         st.launch = launch_rope(p, fp32 != 0, (cudaStream_t) stream);

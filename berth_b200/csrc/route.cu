@@ -604,6 +604,7 @@ void check_routing(const berth_moe_routing* r, int n_experts, int top_k)
     const int gs = n_experts / r->n_group;
     if (top_k > r->topk_group * gs) throw std::runtime_error("moe route: top_k exceeds the experts of topk_group groups");
     if (r->group_score == 1 && gs < 2) throw std::runtime_error("moe route: the sum of two best needs groups of at least two experts");
+    check_aligned(r->selection_bias, 4, "moe route: selection_bias");
     if (!std::isfinite(r->scale)) throw std::runtime_error("moe route: scale must be finite");
 }
 
@@ -659,6 +660,8 @@ extern "C" int berth_moe_route(const void* logits, int logits_fp32, int64_t row_
         if (n_experts < 1 || n_experts > 1024) throw std::runtime_error("moe route: n_experts must be in 1..=1024");
         if (top_k < 1 || top_k > 32 || top_k > n_experts) throw std::runtime_error("moe route: top_k must be in 1..=32 and at most n_experts");
         if (row_stride < n_experts && T > 1) throw std::runtime_error("moe route: row_stride is smaller than n_experts");
+        check_aligned(logits, logits_fp32 ? 4 : 2, "moe route: logits");
+        for (const void* p : {(const void*) topk_idx, (const void*) topk_w}) check_aligned(p, 4, "moe route: a tensor of 32-bit elements");
         const berth_moe_routing r{score, n_group, topk_group, group_score, renormalize, scale, selection_bias};
         check_routing(&r, n_experts, top_k);
         st.launch = route_tokens(logits, logits_fp32 != 0, row_stride, r, topk_idx, topk_w, T, n_experts, top_k, (cudaStream_t) stream);

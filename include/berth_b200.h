@@ -259,8 +259,9 @@ int berth_ops_rms_norm_res_in(const void* x, const void* weight, void* y, void* 
  * as berth_ops_rms_norm_f16 over rows of one head, but not rounded to fp16 before the rotation.
  * One berth_rope_rows describes q or k: x and y of the same type (fp16, or fp32 when fp32 != 0), element strides between
  * tokens and heads for each, so that rows may be columns of a wider buffer or slots of a cache; the head_dim elements
- * of a head are contiguous.  y may be x itself (with x's strides); any other overlap of outputs with inputs, or of two
- * heads of an output, is undefined.  k may be NULL.  norm of q and of k are independent of each other.
+ * of a head are contiguous.  y may be x itself (with x's strides); any other overlap of outputs with inputs, or of q's
+ * output with k's, is undefined.  The larger stride of an output has to step over all that lies along the smaller one.
+ * k may be NULL.  norm of q and of k are independent of each other.
  * positions int32 [n_tokens], any value; inv_freq fp64 [rot_dim / 2]; both device memory.  head_dim up to 512, rot_dim
  * even and at most head_dim.  Rows whose pointers and strides are multiples of 16 bytes take the wide accesses.
  * Touches nothing but the tensors; launches on different streams are independent. */

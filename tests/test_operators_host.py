@@ -184,3 +184,38 @@ def test_reference_rope_by_hand():
     x = np.array([[[1.0, 0.0, 5.0]]])
     out, _ = refs.rope(x, np.array([1]), np.array([math.pi / 2]), True, 2.0, None, 0.0, 0.0)
     assert np.allclose(out, [[[0.0, 2.0, 5.0]]])
+
+
+# ------------------------------------------------------------------ pointers off their elements' boundaries, outputs that overlap
+
+@pytest.mark.parametrize("name", ["logits", "bias", "idx", "w"])
+def test_route_refuses_unaligned_pointers(lib, name):
+    a = {**ROUTE, name: P + 1 if name == "logits" else P + 2}
+    for f32 in (0, 1) if name == "logits" else (1,):
+        rc = lib.berth_moe_route(a["logits"], f32, a["ld"], a["bias"], a["idx"], a["w"], a["T"], a["E"], a["k"], a["score"], a["groups"], a["keep"],
+                                 a["gs"], a["renorm"], a["scale"], None)
+        assert rc == -1 and "not aligned" in moe.last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(q=_rows(x=P + 1)), dict(q=_rows(y=P + 1)), dict(k=_rows(norm=P + 1)), dict(pos=P + 2), dict(f=P + 4),
+                                 dict(q=_rows(x=P + 2), f32=1)])
+def test_rope_refuses_unaligned_pointers(lib, bad):
+    a = {**dict(q=_rows(), k=_rows(), pos=P, f=P, f32=0), **bad}
+    assert lib.berth_ops_rope(a["q"], a["k"], a["pos"], a["f"], 3, 64, 64, 0, 1.0, 1e-6, 0.0, a["f32"], None) == -1
+    assert "not aligned" in ops.last_error()
+
+
+@pytest.mark.parametrize("name,off", [("logits", 2), ("tokens", 2), ("lp", 1), ("rank", 2), ("h", 3), ("ti", 2), ("tl", 2)])
+def test_logprobs_refuses_unaligned_pointers(lib, name, off):
+    a = {**LOGPROBS, name: P + off}
+    rc = lib.berth_ops_logprobs(a["logits"], a["f32"], a["ld"], a["tokens"], a["inv_temp"], a["lp"], a["rank"], a["h"], a["ti"], a["tl"], a["n"],
+                                a["rows"], a["vocab"], None)
+    assert rc == -1 and "not aligned" in ops.last_error()
+
+
+@pytest.mark.parametrize("yt,yh", [(64, 64), (128, 64), (255, 64), (-128, 64), (64, 128), (64, 191), (64, -191), (0, 64), (256, 0), (100, 100)])
+def test_rope_refuses_outputs_whose_heads_overlap(lib, yt, yh):
+    """Three tokens of four heads of 64 (256 or 192 apart is enough): one stride inside what lies along the other."""
+    q = _rows(x=2 * P, yt=yt, yh=yh)
+    assert lib.berth_ops_rope(q, None, P, P, 3, 64, 64, 0, 1.0, 1e-6, 0.0, 0, None) == -1
+    assert "overlap" in ops.last_error()
