@@ -180,7 +180,7 @@ def bind():
             from . import _bind as module
         except ImportError as exc:
             raise RuntimeError(f"berth_b200/_bind.so cannot be loaded ({exc}): build it with `make -C {CSRC}`") from exc
-        module.init(Error, torch)
+        module.init(Error, torch.Tensor)
         _bind = module
     return _bind
 

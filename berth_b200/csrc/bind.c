@@ -1,7 +1,8 @@
 /* berth_b200._bind: the callers of the operators that take shapes and strides from torch tensors (rope, logprobs, route), in C.
  * A decode step calls them with a few rows at a time, and reading eight tensors and checking them in Python took longer (6 us of
- * 10) than the kernels.  No torch headers: a tensor is asked through its own methods.  Every check is made before the library is
- * called; the library's error becomes berth_b200.kernels.Error, set by init(). */
+ * 10) than the kernels.  No torch headers: a tensor is read through the C function that torch.Tensor publishes for this (DLPack's
+ * exchange interface, version 1; asking eight tensors for five attributes each took 2 us).  Every check is made before the library
+ * is called; the library's error becomes berth_b200.kernels.Error, set by init(). */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -9,14 +10,35 @@
 
 #include "../../include/berth_b200.h"
 
-static PyObject *g_error, *g_half, *g_float, *g_double, *g_int32, *g_bfloat16;
-static PyObject *n_data_ptr, *n_get_device, *n_dtype, *n_shape, *n_stride;
+/* DLPack 1.x, the parts in use */
+typedef struct { uint32_t major, minor; } dl_version;
+typedef struct {
+    void* data;
+    int32_t device_type, device_id;
+    int32_t ndim;
+    struct { uint8_t code, bits; uint16_t lanes; } dtype;
+    int64_t *shape, *strides;
+    uint64_t byte_offset;
+} dl_tensor;
+typedef struct {
+    dl_version version;
+    void *previous, *allocate, *managed_from_object, *managed_to_object;
+    int (*tensor_from_object)(void* object, dl_tensor* out);   /* borrowed from the object */
+    void* current_stream;
+} dl_exchange;
+enum { DL_CUDA = 2 };
+
+/* types: DLPack's code (0 integer, 2 float, 4 bfloat) and bits */
+enum { T_INT32 = 0 << 8 | 32, T_HALF = 2 << 8 | 16, T_FLOAT = 2 << 8 | 32, T_DOUBLE = 2 << 8 | 64, T_BFLOAT16 = 4 << 8 | 16 };
+
+static PyObject* g_error;
+static PyTypeObject* g_tensor;
+static const dl_exchange* g_exchange;
 
 typedef struct {
     int given;           /* not None */
-    int nd, dev;
+    int dev, dtype;
     void* ptr;
-    PyObject* dtype;     /* borrowed: the dtypes are torch's own singletons */
     int64_t shape[3], stride[3];
 } tensor;
 
@@ -26,61 +48,52 @@ static int fail(const char* what, const char* name, const char* msg)
     return -1;
 }
 
-static int read_tuple(PyObject* t, int64_t* to, int* n)
-{
-    if (!t) return -1;
-    if (!PyTuple_Check(t)) {
-        Py_DECREF(t);
-        PyErr_SetString(PyExc_TypeError, "a torch tensor is expected");
-        return -1;
-    }
-    const Py_ssize_t count = PyTuple_GET_SIZE(t);
-    *n = (int) count;
-    for (Py_ssize_t i = 0; i < count && i < 3; ++i) to[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(t, i));
-    Py_DECREF(t);
-    return PyErr_Occurred() ? -1 : 0;
-}
-
 /* A tensor of nd dimensions with contiguous innermost elements, or None where it may be. */
 static int read_tensor(PyObject* o, const char* what, const char* name, int nd, int optional, tensor* t)
 {
     t->given = o != Py_None;
     t->ptr = NULL;
-    t->dtype = NULL;
+    t->dtype = -1;
     if (!t->given) return optional ? 0 : fail(what, name, "is missing");
-    int n = 0;
-    if (read_tuple(PyObject_GetAttr(o, n_shape), t->shape, &t->nd) || read_tuple(PyObject_CallMethodNoArgs(o, n_stride), t->stride, &n)) {
+    if (!PyObject_TypeCheck(o, g_tensor)) return fail(what, name, "must be a torch tensor");
+    dl_tensor d;
+    if (g_exchange->tensor_from_object(o, &d)) {
         PyErr_Clear();
-        return fail(what, name, "must be a torch tensor");
+        return fail(what, name, "must be a dense torch tensor");
     }
-    if (t->nd != nd) {
-        PyErr_Format(g_error, "%s: %s must have %d dimensions, got %d", what, name, nd, t->nd);
+    if (d.ndim != nd) {
+        PyErr_Format(g_error, "%s: %s must have %d dimensions, got %d", what, name, nd, (int) d.ndim);
         return -1;
     }
-    PyObject* v = PyObject_GetAttr(o, n_dtype);
-    if (!v) return -1;
-    t->dtype = v;
-    Py_DECREF(v);
-    if (!(v = PyObject_CallMethodNoArgs(o, n_get_device))) return -1;
-    t->dev = (int) PyLong_AsLong(v);
-    Py_DECREF(v);
-    if (t->dev < 0) return fail(what, name, "must be on the CUDA device");
-    if (!(v = PyObject_CallMethodNoArgs(o, n_data_ptr))) return -1;
-    t->ptr = PyLong_AsVoidPtr(v);
-    Py_DECREF(v);
-    if (PyErr_Occurred()) return -1;
+    if (d.device_type != DL_CUDA) return fail(what, name, "must be on the CUDA device");
+    t->dev = d.device_id;
+    t->dtype = d.dtype.lanes == 1 ? d.dtype.code << 8 | d.dtype.bits : -1;
+    t->ptr = (char*) d.data + d.byte_offset;
+    for (int i = 0; i < nd; ++i) {
+        t->shape[i] = d.shape[i];
+        t->stride[i] = d.strides[i];
+    }
     if (t->shape[nd - 1] > 1 && t->stride[nd - 1] != 1) return fail(what, name, "must have contiguous innermost elements");
     return 0;
 }
 
+static const char* type_name(int dtype)
+{
+    switch (dtype) {
+        case T_INT32: return "int32";
+        case T_FLOAT: return "float32";
+        default: return "bfloat16";   /* (what read_flat is asked for) */
+    }
+}
+
 /* A contiguous tensor of the given type and shape (nd 1 or 2), or None. */
-static int read_flat(PyObject* o, const char* what, const char* name, PyObject* dtype, int nd, int64_t rows, int64_t cols, tensor* t)
+static int read_flat(PyObject* o, const char* what, const char* name, int dtype, int nd, int64_t rows, int64_t cols, tensor* t)
 {
     if (read_tensor(o, what, name, nd, 1, t)) return -1;
     if (!t->given) return 0;
     if (t->dtype != dtype || t->shape[0] != rows || (nd == 2 && (t->shape[1] != cols || (rows > 1 && cols > 0 && t->stride[0] != cols)))) {
-        if (nd == 1) PyErr_Format(g_error, "%s: %s must be a contiguous %R tensor of shape (%lld,)", what, name, dtype, (long long) rows);
-        else PyErr_Format(g_error, "%s: %s must be a contiguous %R tensor of shape (%lld, %lld)", what, name, dtype, (long long) rows, (long long) cols);
+        if (nd == 1) PyErr_Format(g_error, "%s: %s must be a contiguous %s tensor of shape (%lld,)", what, name, type_name(dtype), (long long) rows);
+        else PyErr_Format(g_error, "%s: %s must be a contiguous %s tensor of shape (%lld, %lld)", what, name, type_name(dtype), (long long) rows, (long long) cols);
         return -1;
     }
     return 0;
@@ -88,8 +101,8 @@ static int read_flat(PyObject* o, const char* what, const char* name, PyObject* 
 
 static int is_f32(const char* what, const char* name, const tensor* t)
 {
-    if (t->dtype == g_float) return 1;
-    if (t->dtype == g_half) return 0;
+    if (t->dtype == T_FLOAT) return 1;
+    if (t->dtype == T_HALF) return 0;
     return fail(what, name, "must be fp16 or fp32");
 }
 
@@ -141,7 +154,7 @@ static int read_rows(PyObject* x, PyObject* y, PyObject* norm, const char* name,
     if (read_tensor(x, "rope", name, 3, 0, &t[0]) || read_tensor(y, "rope", out_name, 3, 0, &t[1])) return -1;
     if (t[1].dtype != t[0].dtype || t[1].shape[0] != t[0].shape[0] || t[1].shape[1] != t[0].shape[1] || t[1].shape[2] != t[0].shape[2])
         return fail("rope", out_name, "must have the type and shape of its input");
-    if (read_flat(norm, "rope", norm_name, g_bfloat16, 1, t[0].shape[2], 0, &t[2])) return -1;
+    if (read_flat(norm, "rope", norm_name, T_BFLOAT16, 1, t[0].shape[2], 0, &t[2])) return -1;
     if (t[0].shape[0] > INT32_MAX || t[0].shape[1] > INT32_MAX || t[0].shape[2] > INT32_MAX) return fail("rope", name, "is too large");
     rows->x = t[0].ptr;
     rows->y = t[1].ptr;
@@ -176,11 +189,11 @@ static PyObject* py_rope(PyObject* self, PyObject* const* a, Py_ssize_t n)
         return NULL;
     }
     if (read_tensor(a[2], "rope", "positions", 1, 0, &pos) || read_tensor(a[3], "rope", "inv_freq", 1, 0, &freq)) return NULL;
-    if (pos.dtype != g_int32 || pos.shape[0] != q[0].shape[0]) {
+    if (pos.dtype != T_INT32 || pos.shape[0] != q[0].shape[0]) {
         fail("rope", "positions", "must be a contiguous int32 tensor with one entry per token");
         return NULL;
     }
-    if (freq.dtype != g_double || freq.shape[0] > 256) {
+    if (freq.dtype != T_DOUBLE || freq.shape[0] > 256) {
         fail("rope", "inv_freq", "must be a contiguous float64 tensor of at most 256 entries");
         return NULL;
     }
@@ -216,8 +229,8 @@ static PyObject* py_logprobs(PyObject* self, PyObject* const* a, Py_ssize_t n)
         PyErr_Format(g_error, "logprobs: vocab %d exceeds the %lld columns of logits", vocab, (long long) x.shape[1]);
         return NULL;
     }
-    if (read_flat(a[1], what, "tokens", g_int32, 1, rows, 0, &token) || read_flat(a[2], what, "logprob", g_float, 1, rows, 0, &lp) ||
-        read_flat(a[3], what, "rank", g_int32, 1, rows, 0, &rank) || read_flat(a[4], what, "entropy", g_float, 1, rows, 0, &entropy))
+    if (read_flat(a[1], what, "tokens", T_INT32, 1, rows, 0, &token) || read_flat(a[2], what, "logprob", T_FLOAT, 1, rows, 0, &lp) ||
+        read_flat(a[3], what, "rank", T_INT32, 1, rows, 0, &rank) || read_flat(a[4], what, "entropy", T_FLOAT, 1, rows, 0, &entropy))
         return NULL;
     int64_t best = 0;
     if ((a[5] == Py_None) != (a[6] == Py_None)) {
@@ -232,7 +245,7 @@ static PyObject* py_logprobs(PyObject* self, PyObject* const* a, Py_ssize_t n)
             fail(what, "top_idx", "is too large");
             return NULL;
         }
-        if (read_flat(a[5], what, "top_idx", g_int32, 2, rows, best, &top) || read_flat(a[6], what, "top_logprob", g_float, 2, rows, best, &top_lp)) return NULL;
+        if (read_flat(a[5], what, "top_idx", T_INT32, 2, rows, best, &top) || read_flat(a[6], what, "top_logprob", T_FLOAT, 2, rows, best, &top_lp)) return NULL;
     }
     const tensor* ts[7] = {&x, &token, &lp, &rank, &entropy, &top, &top_lp};
     if (same_device(what, ts, 7)) return NULL;
@@ -265,8 +278,8 @@ static PyObject* py_route(PyObject* self, PyObject* const* a, Py_ssize_t n)
     const double scale = PyFloat_AsDouble(a[10]);
     void* stream = to_stream(a[11]);
     if (PyErr_Occurred()) return NULL;
-    if (read_flat(a[1], what, "selection_bias", g_float, 1, experts, 0, &bias) || read_flat(a[2], what, "topk_idx", g_int32, 2, rows, k, &idx) ||
-        read_flat(a[3], what, "topk_w", g_float, 2, rows, k, &w))
+    if (read_flat(a[1], what, "selection_bias", T_FLOAT, 1, experts, 0, &bias) || read_flat(a[2], what, "topk_idx", T_INT32, 2, rows, k, &idx) ||
+        read_flat(a[3], what, "topk_w", T_FLOAT, 2, rows, k, &w))
         return NULL;
     const tensor* ts[4] = {&x, &bias, &idx, &w};
     if (same_device(what, ts, 4)) return NULL;
@@ -275,20 +288,25 @@ static PyObject* py_route(PyObject* self, PyObject* const* a, Py_ssize_t n)
                   what, berth_moe_last_error);
 }
 
-/* init(Error, torch): the exception to raise and the types to compare with */
+/* init(Error, torch.Tensor): the exception to raise and the class of the tensors */
 static PyObject* py_init(PyObject* self, PyObject* const* a, Py_ssize_t n)
 {
     (void) self;
-    if (n != 2) {
-        PyErr_SetString(PyExc_TypeError, "_bind.init takes (Error, torch)");
+    if (n != 2 || !PyType_Check(a[1])) {
+        PyErr_SetString(PyExc_TypeError, "_bind.init takes (Error, torch.Tensor)");
         return NULL;
     }
-    struct { PyObject** to; const char* name; } types[] = {{&g_half, "float16"}, {&g_float, "float32"}, {&g_double, "float64"}, {&g_int32, "int32"}, {&g_bfloat16, "bfloat16"}};
-    for (int i = 0; i < 5; ++i) {
-        PyObject* v = PyObject_GetAttrString(a[1], types[i].name);
-        if (!v) return NULL;
-        Py_XSETREF(*types[i].to, v);
+    PyObject* capsule = PyObject_GetAttrString(a[1], "__dlpack_c_exchange_api__");
+    if (!capsule) return NULL;
+    const dl_exchange* x = (const dl_exchange*) PyCapsule_GetPointer(capsule, "dlpack_exchange_api");   /* lives as long as torch */
+    Py_DECREF(capsule);
+    if (!x) return NULL;
+    if (x->version.major != 1 || !x->tensor_from_object) {
+        PyErr_SetString(PyExc_ImportError, "torch.Tensor offers no DLPack 1.x exchange interface");
+        return NULL;
     }
+    g_exchange = x;
+    Py_XSETREF(g_tensor, (PyTypeObject*) Py_NewRef(a[1]));
     Py_XSETREF(g_error, Py_NewRef(a[0]));
     Py_RETURN_NONE;
 }
@@ -302,11 +320,5 @@ static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", "Callers of 
 
 PyMODINIT_FUNC PyInit__bind(void)
 {
-    n_data_ptr = PyUnicode_InternFromString("data_ptr");
-    n_get_device = PyUnicode_InternFromString("get_device");
-    n_dtype = PyUnicode_InternFromString("dtype");
-    n_shape = PyUnicode_InternFromString("shape");
-    n_stride = PyUnicode_InternFromString("stride");
-    if (!n_data_ptr || !n_get_device || !n_dtype || !n_shape || !n_stride) return NULL;
     return PyModule_Create(&module);
 }

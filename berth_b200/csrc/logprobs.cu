@@ -704,6 +704,6 @@ extern "C" int berth_ops_logprobs(const void* logits, int logits_fp32, int64_t r
         cudaStream_t cs = (cudaStream_t) stream;
         if (f32) ranks ? launch<true, true>(p, ctas, warps, cs) : launch<true, false>(p, ctas, warps, cs);
         else ranks ? launch<false, true>(p, ctas, warps, cs) : launch<false, false>(p, ctas, warps, cs);
-        st.launch = describe("k_logprobs<%s%s> block=%d grid=%dx%d cluster=%d", f32 ? "float" : "half", ranks ? ",rank" : "", warps * 32, rows, ctas, ctas);
+        st.launch = describe("k_logprobs<", f32 ? "float" : "half", ranks ? ",rank" : "", "> block=", warps * 32, " grid=", rows, "x", ctas, " cluster=", ctas);
     });
 }

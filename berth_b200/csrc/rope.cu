@@ -393,8 +393,8 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     };
     if (f32) typed(0.0f);
     else typed(__half{});
-    return describe("%s<%s%s> block=%d grid=%dx%d tokens=%d lanes=%d", name, f32 ? "float" : "half", norm ? ",norm" : "", kThreads, blocks_x, blocks_y, p.tile,
-                    p.lanes);
+    return describe(name, "<", f32 ? "float" : "half", norm ? ",norm" : "", "> block=", kThreads, " grid=", blocks_x, "x", blocks_y, " tokens=", p.tile,
+                    " lanes=", p.lanes);
 }
 
 }  // namespace

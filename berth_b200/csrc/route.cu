@@ -641,7 +641,7 @@ std::string route_tokens(const void* logits, bool f32, long long ld, const berth
         case 32: go(launch<32>); break;
         default: go(launch<64>); break;   // up to 1024 experts: q <= 64
     }
-    return describe("k_moe_route<%d,%s,%s%s> grid=%d", per, f32 ? "float" : "half", score == kSigmoid ? "sigmoid" : "softmax", by_logit ? "" : ",scores", blocks);
+    return describe("k_moe_route<", per, ",", f32 ? "float" : "half", ",", score == kSigmoid ? "sigmoid" : "softmax", by_logit ? "" : ",scores", "> grid=", blocks);
 }
 
 }  // namespace berth
