@@ -85,12 +85,6 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, int cta)
 }
 __device__ __forceinline__ void peer_store(uint32_t a, unsigned v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 __device__ __forceinline__ void peer_store(uint32_t a, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
-__device__ __forceinline__ unsigned peer_add(uint32_t a, unsigned v)
-{
-    unsigned r;
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(a), "r"(v) : "memory");
-    return r;
-}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
@@ -100,7 +94,6 @@ struct Part {
     float m, z, t;
 };
 __device__ __forceinline__ float redux_max(float v) { float r; asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
-__device__ __forceinline__ float redux_min(float v) { float r; asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 // p, whose maximum is not the one that keeps its 1 out of the sum, relative to the maximum m.
 __device__ __forceinline__ Part beside(Part p, float m, float scale2)
@@ -261,7 +254,7 @@ __device__ __forceinline__ unsigned long long merge_lists(unsigned long long a, 
 template <int WARPS>
 struct Shared {
     unsigned long long keys[kKeys];             // first CTA: every CTA's keys that reach tau, or its list; 0 = none
-    unsigned long long lists[kKeys / 32][32];   // the warps' lists of the slow way; first CTA: the keys, one behind the other
+    alignas(16) unsigned long long lists[kKeys / 32][32];   // the warps' lists of the slow way; first CTA: the keys, one behind the other
     float m[kMaxCluster * WARPS], z[kMaxCluster * WARPS], t[kMaxCluster * WARPS];   // first CTA: the parts of the cluster's warps
     int before[kMaxCluster * WARPS];
     float reach[kMaxCluster * WARPS];           // what logits of every warp of the cluster reach
@@ -304,7 +297,7 @@ __device__ __noinline__ void sorted_lists(Shared<WARPS>& sh, const char* row, co
 // vectors of a thread at a time, while those of the next step are on their way to shared memory.
 // Bound: long rows, instructions (9.2 warp instructions per 32 logits, 70 % of the issue slots) and ex2 (67 % of its pipe) before
 // HBM; few rows, the fixed parts of a call (cluster barriers, the dependent reads of the candidates, the join: 4 to 5 us).
-// 421 x 248320 fp16, 5 alternatives, 48 us (4.4 TB/s), without alternatives 43; 32 x 248320 fp32 12.0 us (2.6 TB/s); 77 x 100003 fp32
+// 421 x 248320 fp16, 5 alternatives, 47.5 us (4.4 TB/s), without alternatives 42.1; 32 x 248320 fp32 12.0 us (2.6 TB/s); 77 x 100003 fp32
 // 9.4 us (3.3 TB/s); 1 x 248320 fp32 8.2 us.
 template <bool F32, bool RANK, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const LogprobParams p)
@@ -489,33 +482,40 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
     // ---- the candidates for the n best
     if (p.top_n > 0) {
         // up to 32 or 64 different logits that the row reaches, of as many groups of warps or of the warps' largest threads; tau: the
-        // n-th of them, by rounds, or for a larger n close below it by bisection.  With 32 groups an n of 32 would let in all
-        // that exceeds the least of them, some 130 logits and now and then 300: 16 rows of 15390 fp32 11.8 us, now 6.5.
-        float x = -INFINITY, tau = 0.f;
+        // n-th of them, the largest that n of them reach (counted by every lane for its own one or two: n rounds of taking the
+        // largest, and bisection for a larger n, took longer, 421 x 248320 fp16 48.4 us, now 47.5).  With 32 groups an n of 32
+        // would let in all that exceeds the least of them, some 130 logits and now and then 300: 16 rows of 15390 fp32 11.8 us, now 6.5.
         const int values = warps << k_shift;
+        float* const reached = reinterpret_cast<float*>(sh.lists[warp]);
+        float x = -INFINITY, y = -INFINITY;
+        int nx = 0, ny = 0;
         if (many) {
-            float y = -INFINITY;
             for (int i = lane; i < values; i += 64) {
                 x = fmaxf(x, sh.reach[i]);
                 y = fmaxf(y, sh.reach[i + 32]);
             }
-            const unsigned a = order_bits(x), b = order_bits(y);
-            unsigned lo = __reduce_min_sync(dq::kFull, min(a, b)), hi = __reduce_max_sync(dq::kFull, max(a, b));
-            for (int i = 0; i < 10 && lo < hi; ++i) {
-                const unsigned mid = lo + (hi - lo + 1) / 2;
-                if (__popc(__ballot_sync(dq::kFull, a >= mid)) + __popc(__ballot_sync(dq::kFull, b >= mid)) >= p.top_n) lo = mid;
-                else hi = mid - 1;
-            }
-            tau = key_value((unsigned long long) lo << 32);
+            reached[lane + 32] = y;
         } else {
             for (int i = lane; i < values; i += 32) x = fmaxf(x, sh.reach[i]);
-            const bool down = p.top_n <= 16;   // from the nearer end
-            const float gone = down ? -INFINITY : INFINITY;
-            for (int i = down ? p.top_n : 33 - p.top_n; i > 0; --i) {
-                tau = down ? redux_max(x) : redux_min(x);
-                if (lane == __ffs(__ballot_sync(dq::kFull, x == tau)) - 1) x = gone;
+        }
+        reached[lane] = x;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(reached + i);
+            nx += (o.x >= x) + (o.y >= x) + (o.z >= x) + (o.w >= x);
+            if (many) ny += (o.x >= y) + (o.y >= y) + (o.z >= y) + (o.w >= y);
+        }
+        if (many) {
+#pragma unroll
+            for (int i = 32; i < 64; i += 4) {
+                const float4 o = *reinterpret_cast<const float4*>(reached + i);
+                nx += (o.x >= x) + (o.y >= x) + (o.z >= x) + (o.w >= x);
+                ny += (o.x >= y) + (o.y >= y) + (o.z >= y) + (o.w >= y);
             }
         }
+        __syncwarp();
+        const float tau = redux_max(fmaxf(nx >= p.top_n ? x : -INFINITY, many && ny >= p.top_n ? y : -INFINITY));
 
         const int room = kKeys / ctas;
         const uint32_t keys0 = peer_addr(&sh.keys[cta * room], 0);
@@ -591,14 +591,24 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
     }
     if (p.top_n == 0) return;
     unsigned long long* list = &sh.lists[0][0];
-    for (int i = tid; i < kKeys; i += kThreads) {
-        const unsigned long long key = sh.keys[i];
-        const unsigned has = __ballot_sync(dq::kFull, key != 0);
-        if (has) {
-            unsigned base = 0;
-            if (lane == 0) base = atomicAdd(&sh.n_keys, __popc(has));
-            base = __shfl_sync(dq::kFull, base, 0) + __popc(has & ((1u << lane) - 1));
-            if (key != 0) list[base] = key;
+    {
+        constexpr int kMine = kKeys / kThreads;   // a thread's keys; one warp's lie together in the list, whatever their order
+        unsigned long long key[kMine];
+        unsigned has[kMine], count = 0, base = 0;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            key[i] = sh.keys[tid + i * kThreads];
+            has[i] = __ballot_sync(dq::kFull, key[i] != 0);
+            count += __popc(has[i]);
+        }
+        if (count) {
+            if (lane == 0) base = atomicAdd(&sh.n_keys, count);
+            base = __shfl_sync(dq::kFull, base, 0);
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                if (key[i] != 0) list[base + __popc(has[i] & ((1u << lane) - 1))] = key[i];
+                base += __popc(has[i]);
+            }
         }
     }
     __syncthreads();
@@ -607,8 +617,11 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const Logpr
         const int k = base + (tid >> 2);
         const unsigned long long key = k < n_keys ? list[k] : 0;
         int place = 0;
-#pragma unroll 4
-        for (int i = quarter; i < n_keys; i += 4) place += list[i] > key;
+#pragma unroll 1
+        for (int i = 4 * quarter; i < n_keys; i += 16) {
+            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(list + i), b = *reinterpret_cast<const ulonglong2*>(list + i + 2);
+            place += (a.x > key) + (i + 1 < n_keys && a.y > key) + (i + 2 < n_keys && b.x > key) + (i + 3 < n_keys && b.y > key);
+        }
         place += __shfl_xor_sync(dq::kFull, place, 1);
         place += __shfl_xor_sync(dq::kFull, place, 2);
         if (quarter == 0 && key != 0 && place < p.top_n) {
