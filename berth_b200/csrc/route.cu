@@ -205,23 +205,35 @@ __device__ __forceinline__ unsigned third_key(const unsigned (&key)[PER], unsign
     for (int off = 1; off < lanes; off <<= 1) k3 = max(k3, __shfl_xor_sync(dq::kFull, k3, off));
     return k3;
 }
-// The choice score of expert e in 64 bits (not for softmax, which needs its sum).
+// What a softmax under a bias needs in 64 bits: the sum of a finite row's exp(l - m).
+template <bool F32>
+__device__ __noinline__ double sum64(const void* row, int cnt, int base, double m)
+{
+    double z = 0.0;
+#pragma unroll 1
+    for (int i = 0; i < cnt; ++i) z += exp(double(logit_at<F32>(row, base + i)) - m);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) z += __shfl_xor_sync(dq::kFull, z, off);
+    return z;
+}
+// The choice score of expert e in 64 bits (softmax: m and z of the row).
 template <bool F32, int ORDER>
-__device__ __forceinline__ double score64(const void* row, int e, const RouteParams& p)
+__device__ __forceinline__ double score64(const void* row, int e, double m, double z, const RouteParams& p)
 {
     const double v = logit_at<F32>(row, e);
-    return ORDER == kByLogit ? v : 1.0 / (1.0 + exp(-v)) + (p.bias ? double(p.bias[e]) : 0.0);
+    if (ORDER == kByLogit) return v;
+    return (ORDER == kSoftmax ? exp(v - m) / z : 1.0 / (1.0 + exp(-v))) + (p.bias ? double(p.bias[e]) : 0.0);
 }
 // Whether this lane's group is kept, by the scores of the groups' two best experts (keys k1, k2; two lanes of a group or more).
 template <bool F32, int ORDER, int LOG_PER>
-__device__ __noinline__ bool groups_again(const void* row, unsigned k1, unsigned k2, int log_p, bool top2, const RouteParams& p)
+__device__ __noinline__ bool groups_again(const void* row, unsigned k1, unsigned k2, int log_p, bool top2, double m, double z, const RouteParams& p)
 {
     const int lane = threadIdx.x & 31, g = lane >> log_p, member = lane & (p.P - 1);
     double c = -INFINITY;
     const unsigned key = member == 0 ? k1 : k2;
     if (g < p.G && member < 2 && key != 0u) {   // (groups of one expert: no second key)
         const int owner = 31 - int(key >> LOG_PER & 31u);
-        c = score64<F32, ORDER>(row, (owner >> log_p) * p.gs + (owner & (p.P - 1)) * p.q + ((1 << LOG_PER) - 1 - int(key & ((1u << LOG_PER) - 1))), p);
+        c = score64<F32, ORDER>(row, (owner >> log_p) * p.gs + (owner & (p.P - 1)) * p.q + ((1 << LOG_PER) - 1 - int(key & ((1u << LOG_PER) - 1))), m, z, p);
     }
     const double other = __shfl_xor_sync(dq::kFull, c, 1);
     const double worth = __shfl_sync(dq::kFull, top2 ? c + other : fmax(c, other), lane & ~(p.P - 1));
@@ -247,11 +259,11 @@ constexpr int min_blocks(int per) { return per < 8 ? 8 : per == 8 ? 6 : per == 1
 //   fp16 logits by themselves: the order of their bits, which have room for the place: exact.
 // Where two neighbours in the order (the first expert not chosen among them) lie closer than both scores' errors and the steps, the
 // k + 1 first are ordered anew in 64 bits, one a lane; so are the groups by their two best experts, where the last one kept and the
-// first one dropped lie as close.  The whole choice is repeated where that may not be enough (a third one as close, a softmax under
-// a bias) and for a row that has an infinite or NaN logit.
+// first one dropped lie as close.  The whole choice is repeated where that may not be enough (a third one as close) and for a row that
+// has an infinite or NaN logit.
 // Errors of c = s + b in units of 2^-24: sigmoid, s (1 - s) (1.5 |l| + 4) for exp and 3 for sum and reciprocal, below 4.5 each;
-// softmax, s (2.5 |l - m| + 7) <= 9 each and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below 2 (28 + PER) for a pair; the sum
-// with the bias, and the bias less the least, half a step of at most the span each.
+// softmax, s (2.5 |l - m| + 7) <= 9 S each, S the row's largest, and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below
+// 2 (28 + PER) S for a pair; the sum with the bias, and the bias less the least, half a step of at most the span each.
 // Bound: instructions, half of them on the half-rate integer pipe, and their latency: 16384 tokens of 256 experts, 8 groups, 8 chosen
 // 13.8 us (17.8 MB would be 2.7), of which 2.5 are a call's least; all of it in 64 bits 57 us.
 template <int PER, bool F32, int ORDER>
@@ -329,8 +341,9 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
     const bool never = !(span < 1e30f);
     const float scale = ((1 << kSteps) - 4) / span;
     // how close two choice scores, or two groups' scores, may lie before 64 bits decide: their errors, and two steps of each key
-    const float error = ORDER == kByLogit ? 0.f : kUnit * ((ORDER == kSigmoid ? 9.f : 2.f * (28 + PER)) + 4.f * span);
-    const unsigned near = kExact ? 0u : unsigned(error * scale) + 4u;
+    // (softmax: of the row's largest score, once that is known)
+    unsigned near = kExact ? 0u : unsigned(ORDER == kByLogit ? 0.f : kUnit * ((ORDER == kSigmoid ? 9.f : 0.f) + 4.f * span) * scale) + 4u;
+    const unsigned near_bias = near;
 
     if constexpr (kSorted) {
         for (int r = 0; r < kRuns; ++r)
@@ -371,6 +384,7 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
             z = warp_sum(z);
         }
         const float inv = ORDER == kSoftmax ? rcp(z) : 0.f;
+        if constexpr (ORDER == kSoftmax) near = near_bias + unsigned(kUnit * 2.1f * (28 + PER) * inv * scale) + 1u;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (ORDER == kByLogit) c[i] = l[i];
@@ -449,12 +463,10 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
                 // too close for the keys: the groups anew by their two best experts' scores in 64 bits, one a lane, where no group has
                 // a third one that could be the second
                 unsigned k3 = 0;
-                if constexpr (ORDER != kSoftmax && kSorted) {
-                    k3 = third_key<PER>(key, k2, p.P);
-                }
-                const bool apart = ORDER != kSoftmax && kSorted && p.P > 1 && (g >= p.G || k3 == 0u || (k2 >> kPlace) - (k3 >> kPlace) > near) &&
+                if constexpr (kSorted) k3 = third_key<PER>(key, k2, p.P);
+                const bool apart = kSorted && p.P > 1 && (g >= p.G || k3 == 0u || (k2 >> kPlace) - (k3 >> kPlace) > near) &&
                                    (ORDER != kByLogit || g >= p.G || ((k2 >> kPlace) & kScore) > 4u);
-                if (__all_sync(dq::kFull, apart) && !__any_sync(dq::kFull, unsure)) open = groups_again<F32, ORDER, Log2<PER>::v>(row, k1, k2, log_p, top2, p);
+                if (__all_sync(dq::kFull, apart) && !__any_sync(dq::kFull, unsure)) open = groups_again<F32, ORDER, Log2<PER>::v>(row, k1, k2, log_p, top2, m, ORDER == kSoftmax ? sum64<F32>(row, cnt, base, m) : 0.0, p);
                 else unsure = true;
             }
             if (ORDER == kByLogit && F32) unsure |= (top >> kPlace & kScore) <= 4u;   // (below the 32 of the logits, the steps end)
@@ -526,11 +538,12 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
             if (ORDER == kByLogit) unsure |= lane < p.k && (won >> kPlace & kScore) <= 4u;
             if (__any_sync(dq::kFull, close)) {
                 // neighbours too close for the keys: the k + 1 first anew by their scores in 64 bits, one a lane, where the one
-                // behind them cannot be among the k (and softmax has its sum in 32 bits: not here)
-                const bool apart = ORDER != kSoftmax && p.k < 32 && (beyond == 0u || (last >> kPlace) - (beyond >> kPlace) > near);
+                // behind them cannot be among the k
+                const bool apart = p.k < 32 && (beyond == 0u || (last >> kPlace) - (beyond >> kPlace) > near);
                 if (apart && !__any_sync(dq::kFull, unsure)) {
                     const bool one = lane < p.k || (lane == p.k && won != 0u);
-                    const double c = one ? score64<F32, ORDER>(row, mine, p) : -INFINITY;
+                    const double sum = ORDER == kSoftmax ? sum64<F32>(row, cnt, base, m) : 0.0;
+                    const double c = one ? score64<F32, ORDER>(row, mine, m, sum, p) : -INFINITY;
                     int before = 0;
                     for (int j = 0; j <= p.k; ++j) {
                         const double oc = __shfl_sync(dq::kFull, c, j);

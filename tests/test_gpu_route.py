@@ -136,6 +136,29 @@ def test_many_tokens_every_choice_equal(T):
     assert np.allclose(w, 2.5 * sel / sel.sum(1, keepdims=True), rtol=80 * 2.0 ** -24, atol=0)
 
 
+@pytest.mark.parametrize("groups,keep,gs", [(1, 1, "max"), (4, 3, "top2"), (4, 2, "max")])
+@pytest.mark.parametrize("E,f32", [(88, True), (88, False), (256, True), (320, True)])
+def test_many_tokens_softmax_under_a_bias(groups, keep, gs, E, f32):
+    """Scores and bias of one size, so that of thousands of tokens some have neighbours that 32 bits cannot tell; a vectorised
+    reference.  Half of the tokens are sharp: there the scores' errors are those of values near 1."""
+    T, k = 6000, 9
+    r = np.random.default_rng(E + groups)
+    l = r.normal(0, 1, (T, E)) * np.where(np.arange(T) % 2, 4.0, 1.0)[:, None]
+    l = l.astype(np.float32 if f32 else np.float16)
+    b = (r.normal(0, 0.5, E) / E).astype(np.float32)
+    idx, _ = _run(l, b, k, score="softmax", groups=groups, keep=keep, group_score=gs, scale=1.0)
+    x = l.astype(np.float64)
+    s = np.exp(x - x.max(1, keepdims=True))
+    c = s / s.sum(1, keepdims=True) + b.astype(np.float64)
+    best = np.sort(c.reshape(T, groups, -1), axis=2)
+    worth = best[:, :, -2:].sum(2) if gs == "top2" else best[:, :, -1]
+    kept = np.argsort(-worth, axis=1, kind="stable")[:, :keep]
+    allowed = np.zeros((T, groups), bool)
+    np.put_along_axis(allowed, kept, True, 1)
+    want = np.argsort(-np.where(np.repeat(allowed, E // groups, 1), c, -np.inf), axis=1, kind="stable")[:, :k]
+    assert (idx == want).all()
+
+
 def test_route_captured_and_on_two_streams():
     """A captured and replayed call follows its inputs; two streams at once share nothing."""
     l, b = _make(21, 300, 128)
