@@ -5,6 +5,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
+#include <utility>
 
 namespace berth {
 namespace {
@@ -39,51 +41,69 @@ __device__ __forceinline__ float2 turn(int position, double inv_freq, float fact
     return make_float2(c * factor, s * factor);
 }
 
-// Sixteen elements of a head, as two pieces of eight (kHalf: i.. and i + rot / 2.. , so that a lane holds both elements of its
-// eight pairs), in 16-byte accesses.
-template <typename T> struct Piece;
-template <> struct Piece<__half> {
-    uint4 v;
-    __device__ __forceinline__ void load(const __half* p) { v = *reinterpret_cast<const uint4*>(p); }
+// N elements of a head in one access of the widest kind (two for 8 fp32).
+template <typename T, int N> struct Piece;
+template <int N> struct Piece<__half, N> {
+    using V = typename std::conditional<N == 8, uint4, typename std::conditional<N == 4, uint2, uint32_t>::type>::type;
+    V v;
+    __device__ __forceinline__ void load(const __half* p) { v = *reinterpret_cast<const V*>(p); }
     __device__ __forceinline__ void get(float* x) const
     {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < N / 2; ++i) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
             x[2 * i] = f.x; x[2 * i + 1] = f.y;
         }
     }
     static __device__ __forceinline__ void store(__half* p, const float* x)
     {
-        uint32_t w[4];
+        V v;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < N / 2; ++i) {
             const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<V*>(p) = v;
     }
 };
-template <> struct Piece<float> {
-    float4 v[2];
-    __device__ __forceinline__ void load(const float* p) { v[0] = reinterpret_cast<const float4*>(p)[0]; v[1] = reinterpret_cast<const float4*>(p)[1]; }
+template <int N> struct Piece<float, N> {
+    using V = typename std::conditional<N == 2, float2, float4>::type;
+    static constexpr int kEach = N == 2 ? 2 : 4, kParts = N / kEach;
+    V v[kParts];
+    __device__ __forceinline__ void load(const float* p)
+    {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) v[i] = reinterpret_cast<const V*>(p)[i];
+    }
     __device__ __forceinline__ void get(float* x) const
     {
-        x[0] = v[0].x; x[1] = v[0].y; x[2] = v[0].z; x[3] = v[0].w; x[4] = v[1].x; x[5] = v[1].y; x[6] = v[1].z; x[7] = v[1].w;
+        const float* e = reinterpret_cast<const float*>(v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = e[i];
     }
     static __device__ __forceinline__ void store(float* p, const float* x)
     {
-        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            V v;
+            float* e = reinterpret_cast<float*>(&v);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) e[j] = x[i * kEach + j];
+            reinterpret_cast<V*>(p)[i] = v;
+        }
     }
 };
-__device__ __forceinline__ uint4 weights8(const void* w, int at) { return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + at); }
-__device__ __forceinline__ void norm8(float* x, const uint4& v, float rinv, float bias)
+// N of the norm's weights, bfloat16, at an offset of whole pieces.
+template <int N>
+__device__ __forceinline__ void norm_piece(float* x, const void* w, int at, float rinv, float bias)
 {
-    const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+    using V = typename Piece<__half, N>::V;
+    const V v = *reinterpret_cast<const V*>(static_cast<const uint16_t*>(w) + at);
+    const uint32_t* h = reinterpret_cast<const uint32_t*>(&v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N / 2; ++i) {
         x[2 * i] = x[2 * i] * rinv * (__uint_as_float(h[i] << 16) + bias);
         x[2 * i + 1] = x[2 * i + 1] * rinv * (__uint_as_float(h[i] & 0xffff0000u) + bias);
     }
@@ -93,29 +113,35 @@ constexpr int kThreads = 128, kTable = 2048;   // cos / sin pairs a block holds
 
 // A block takes p.tile tokens: it fills a table of their cos and sin (one thread per pair and token, 64-bit angles), then groups of
 // p.lanes lanes walk the heads, each lane sixteen elements of a head.  A group stays with its token, so a lane's eight pairs of cos
-// and sin stay in registers.  kHalf / kNeighbours: wide accesses, rotated pieces of whole eights.
-enum { kHalf = 0, kNeighbours = 1 };
-template <typename T, int MODE, bool NORM>
+// and sin stay in registers.  N > 0: halves of the rotated part in pieces of N elements (the widest of 8, 4, 2 that divides rot / 2), of
+// which a lane holds both sides, so that a pair meets in a lane; kNeighbours: any pairs, in pieces of 8.
+constexpr int kNeighbours = 0;
+template <typename T, int N, bool NORM>
 __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
 {
+    constexpr int kPiece = N == kNeighbours ? 8 : N, kPairs = 8 / kPiece;   // elements of a piece; pairs of pieces of a lane
     __shared__ __align__(16) float2 table[kTable];
     pdl_trigger();
     pdl_wait();
     const int tid = threadIdx.x, heads = p.r[0].heads + p.r[1].heads;
     const int group = tid / p.lanes, lane = tid % p.lanes, groups_per_token = kThreads / p.lanes / p.tile;
     const int slot = group / groups_per_token, t0 = blockIdx.x * p.tile, t = t0 + slot;
-    // the lane's pieces: offsets of eight elements, -1 = none
-    const int turning = MODE == kHalf ? p.half_rot / 8 : (p.rot + 15) / 16;   // lanes that turn something
-    int at[2];
-    if (lane < turning) {
-        at[0] = MODE == kHalf ? 8 * lane : 16 * lane;
-        at[1] = at[0] + (MODE == kHalf ? p.half_rot : 8);
-    } else {
-        at[0] = (MODE == kHalf ? p.rot : 16 * turning) + 16 * (lane - turning);
-        at[1] = at[0] + 8;
+    // the pairs of pieces j * lanes + lane: first those that turn something, then what is passed on.  Offsets, -1 = none.
+    const int turning = N == kNeighbours ? (p.rot + 15) / 16 : p.half_rot / kPiece;
+    int at[2][kPairs];
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+        const int q = j * p.lanes + lane;
+        if (q < turning) {
+            at[0][j] = N == kNeighbours ? 16 * q : kPiece * q;
+            at[1][j] = at[0][j] + (N == kNeighbours ? 8 : p.half_rot);
+        } else {
+            at[0][j] = (N == kNeighbours ? 16 * turning : p.rot) + 2 * kPiece * (q - turning);
+            at[1][j] = at[0][j] + kPiece;
+        }
+        if (at[0][j] >= p.dim) at[0][j] = -1;
+        if (at[1][j] >= p.dim) at[1][j] = -1;
     }
-    if (at[0] >= p.dim) at[0] = -1;
-    if (at[1] >= p.dim) at[1] = -1;
 
     auto rows_of = [&](int h, const T*& x, T*& y, const void*& norm) {
         const berth_rope_rows& r = p.r[h >= p.r[0].heads];
@@ -130,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
     // one: 30.2), one where there is a norm (35.1 us, two: 38.2) or fp32 (4096 tokens 32.6 us, two: 33.6)
     constexpr int kAhead = NORM || sizeof(T) == 4 ? 1 : 2;
     struct Head {
-        Piece<T> in[2];
+        Piece<T, kPiece> in[2][kPairs];
         T* y;
         const void* norm;
     } ahead[kAhead];
@@ -145,7 +171,9 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (at[i] >= 0) to.in[i].load(x + at[i]);
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j)
+                    if (at[i][j] >= 0) to.in[i][j].load(x + at[i][j]);
         }
     };
 #pragma unroll
@@ -155,13 +183,14 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
         if (t0 + s < p.tokens) table[i] = turn(p.positions[t0 + s], p.inv_freq[i - s * p.half_rot], p.factor);
     }
     __syncthreads();
-    float2 cs[8];
-    if (lane < turning) {
+    float2 cs[8];   // of a lane's pairs; pairs that do not turn have none
 #pragma unroll
-        for (int i = 0; i < 8; ++i) if (8 * lane + i < p.half_rot) cs[i] = table[slot * p.half_rot + 8 * lane + i];
+    for (int i = 0; i < 8; ++i) {
+        const int pair = (i / kPiece * p.lanes + lane) * kPiece + i % kPiece;
+        if (pair < p.half_rot) cs[i] = table[slot * p.half_rot + pair];
     }
     auto work = [&](Head& now) {
-        float v[16];
+        float v[16];   // first sides, second sides
         const bool live = t < p.tokens && h < heads;
         T* to = nullptr;
         const void* w = nullptr;
@@ -174,11 +203,13 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (live && at[i] >= 0) now.in[i].get(v + 8 * i);
-            else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[8 * i + j] = 0.f;
-            }
+            for (int j = 0; j < kPairs; ++j)
+                if (live && at[i][j] >= 0) now.in[i][j].get(v + 8 * i + kPiece * j);
+                else {
+#pragma unroll
+                    for (int e = 0; e < kPiece; ++e) v[8 * i + kPiece * j + e] = 0.f;
+                }
         fetch(now, h + kAhead * step);
         h += step;
         if constexpr (NORM) {
@@ -190,23 +221,25 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
                 const float rinv = rsqrtf(s / float(p.dim) + p.eps);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (at[i] >= 0) norm8(v + 8 * i, weights8(w, at[i]), rinv, p.bias);
+#pragma unroll
+                    for (int j = 0; j < kPairs; ++j)
+                        if (at[i][j] >= 0) norm_piece<kPiece>(v + 8 * i + kPiece * j, w, at[i][j], rinv, p.bias);
             }
         }
-        if (lane < turning) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (MODE == kNeighbours && 8 * lane + i >= p.half_rot) break;   // the rest of the last lane is passed on
-                float &a = MODE == kHalf ? v[i] : v[2 * i], &b = MODE == kHalf ? v[8 + i] : v[2 * i + 1];
-                const float a0 = a, b0 = b;
-                a = a0 * cs[i].x - b0 * cs[i].y;
-                b = b0 * cs[i].x + a0 * cs[i].y;
-            }
+        for (int i = 0; i < 8; ++i) {
+            if (N == kNeighbours ? 8 * lane + i >= p.half_rot : i / kPiece * p.lanes + lane >= turning) continue;   // passed on
+            float &a = N == kNeighbours ? v[2 * i] : v[i], &b = N == kNeighbours ? v[2 * i + 1] : v[8 + i];
+            const float a0 = a, b0 = b;
+            a = a0 * cs[i].x - b0 * cs[i].y;
+            b = b0 * cs[i].x + a0 * cs[i].y;
         }
         if (live) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (at[i] >= 0) Piece<T>::store(to + at[i], v + 8 * i);
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j)
+                    if (at[i][j] >= 0) Piece<T, kPiece>::store(to + at[i][j], v + 8 * i + kPiece * j);
         }
     };
     // every lane of a warp walks alike, so that the norm's sums meet
@@ -266,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_rope_any(const RopeParams p, bo
         T* y = static_cast<T*>(r.y) + t * r.y_token + hh * r.y_head;
         float v[16];
         if (wide && live && e0 + 16 <= p.dim) {
-            Piece<T> a, b;
+            Piece<T, 8> a, b;
             a.load(x + e0);
             b.load(x + e0 + 8);
             a.get(v);
@@ -283,8 +316,8 @@ __global__ void __launch_bounds__(kThreads, 5) k_rope_any(const RopeParams p, bo
             if (live && r.norm) {
                 const float rinv = rsqrtf(s / float(p.dim) + p.eps);
                 if (wide && e0 + 16 <= p.dim) {
-                    norm8(v, weights8(r.norm, e0), rinv, p.bias);
-                    norm8(v + 8, weights8(r.norm, e0 + 8), rinv, p.bias);
+                    norm_piece<8>(v, r.norm, e0, rinv, p.bias);
+                    norm_piece<8>(v + 8, r.norm, e0 + 8, rinv, p.bias);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -311,8 +344,8 @@ __global__ void __launch_bounds__(kThreads, 5) k_rope_any(const RopeParams p, bo
         }
         if (!live) continue;
         if (wide && e0 + 16 <= p.dim) {
-            Piece<T>::store(y + e0, v);
-            Piece<T>::store(y + e0 + 8, v + 8);
+            Piece<T, 8>::store(y + e0, v);
+            Piece<T, 8>::store(y + e0 + 8, v + 8);
         } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -360,13 +393,14 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
 {
     const int heads = p.r[0].heads + p.r[1].heads;
     const bool wide = wide_rows(p, f32 ? 4 : 2) && p.dim % 8 == 0, norm = p.r[0].norm || p.r[1].norm;
-    const bool eights = wide && (p.interleaved ? p.rot % 8 == 0 : p.half_rot % 8 == 0);
-    // lanes: pieces that turn, then what is passed on
+    // pieces of a half: the widest that divide it; neighbours meet in one piece whatever their number
+    const int piece = !wide ? 0 : p.interleaved || p.half_rot % 8 == 0 ? 8 : p.half_rot % 4 == 0 ? 4 : p.half_rot % 2 == 0 ? 2 : 0;
+    // lanes: pieces that turn, then what is passed on (of which kNeighbours leaves a piece of a lane empty at most)
     int units = (p.dim + 15) / 16;
-    if (eights) {
-        const int turning = p.interleaved ? (p.rot + 15) / 16 : p.half_rot / 8, passed = p.interleaved ? 16 * turning : p.rot;
-        units = turning + std::max(0, (p.dim - passed + 15) / 16);
-    }
+    if (piece && p.interleaved) {
+        const int turning = (p.rot + 15) / 16;
+        units = turning + std::max(0, (p.dim - 16 * turning + 15) / 16);
+    } else if (piece == 8) units = p.half_rot / 8 + (p.dim - p.rot + 15) / 16;
     p.lanes = 1;
     while (p.lanes < units) p.lanes *= 2;
     const int groups = kThreads / p.lanes;
@@ -387,14 +421,20 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     };
     auto typed = [&](auto zero) {
         using T = decltype(zero);
-        if (!eights) norm ? go(k_rope_any<T, true>, "k_rope_any", wide) : go(k_rope_any<T, false>, "k_rope_any", wide);
+        auto halves = [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            norm ? go(k_rope<T, N, true>, "k_rope_half") : go(k_rope<T, N, false>, "k_rope_half");
+        };
+        if (!piece) norm ? go(k_rope_any<T, true>, "k_rope_any", wide) : go(k_rope_any<T, false>, "k_rope_any", wide);
         else if (p.interleaved) norm ? go(k_rope<T, kNeighbours, true>, "k_rope_neighbours") : go(k_rope<T, kNeighbours, false>, "k_rope_neighbours");
-        else norm ? go(k_rope<T, kHalf, true>, "k_rope_half") : go(k_rope<T, kHalf, false>, "k_rope_half");
+        else if (piece == 8) halves(std::integral_constant<int, 8>{});
+        else if (piece == 4) halves(std::integral_constant<int, 4>{});
+        else halves(std::integral_constant<int, 2>{});
     };
     if (f32) typed(0.0f);
     else typed(__half{});
     return describe(name, "<", f32 ? "float" : "half", norm ? ",norm" : "", "> block=", kThreads, " grid=", blocks_x, "x", blocks_y, " tokens=", p.tile,
-                    " lanes=", p.lanes);
+                    " lanes=", p.lanes, " piece=", piece);
 }
 
 }  // namespace
