@@ -41,7 +41,7 @@ __device__ __forceinline__ float2 turn(int position, double inv_freq, float fact
     return make_float2(c * factor, s * factor);
 }
 
-// N elements of a head in one access of the widest kind (two for 8 fp32).
+// N elements of a head: 16, 8 or 4 bytes in one access (8 fp32 in two).
 template <typename T, int N> struct Piece;
 template <int N> struct Piece<__half, N> {
     using V = typename std::conditional<N == 8, uint4, typename std::conditional<N == 4, uint2, uint32_t>::type>::type;
@@ -69,8 +69,8 @@ template <int N> struct Piece<__half, N> {
     }
 };
 template <int N> struct Piece<float, N> {
-    using V = typename std::conditional<N == 2, float2, float4>::type;
-    static constexpr int kEach = N == 2 ? 2 : 4, kParts = N / kEach;
+    using V = typename std::conditional<N == 1, float, typename std::conditional<N == 2, float2, float4>::type>::type;
+    static constexpr int kEach = N < 4 ? N : 4, kParts = N / kEach;
     V v[kParts];
     __device__ __forceinline__ void load(const float* p)
     {
@@ -99,13 +99,17 @@ template <int N> struct Piece<float, N> {
 template <int N>
 __device__ __forceinline__ void norm_piece(float* x, const void* w, int at, float rinv, float bias)
 {
-    using V = typename Piece<__half, N>::V;
-    const V v = *reinterpret_cast<const V*>(static_cast<const uint16_t*>(w) + at);
-    const uint32_t* h = reinterpret_cast<const uint32_t*>(&v);
+    if constexpr (N == 1) {
+        x[0] = x[0] * rinv * (bf16_at(w, at) + bias);
+    } else {
+        using V = typename Piece<__half, N>::V;
+        const V v = *reinterpret_cast<const V*>(static_cast<const uint16_t*>(w) + at);
+        const uint32_t* h = reinterpret_cast<const uint32_t*>(&v);
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-        x[2 * i] = x[2 * i] * rinv * (__uint_as_float(h[i] << 16) + bias);
-        x[2 * i + 1] = x[2 * i + 1] * rinv * (__uint_as_float(h[i] & 0xffff0000u) + bias);
+        for (int i = 0; i < N / 2; ++i) {
+            x[2 * i] = x[2 * i] * rinv * (__uint_as_float(h[i] << 16) + bias);
+            x[2 * i + 1] = x[2 * i + 1] * rinv * (__uint_as_float(h[i] & 0xffff0000u) + bias);
+        }
     }
 }
 
@@ -113,30 +117,38 @@ constexpr int kThreads = 128, kTable = 2048;   // cos / sin pairs a block holds
 
 // A block takes p.tile tokens: it fills a table of their cos and sin (one thread per pair and token, 64-bit angles), then groups of
 // p.lanes lanes walk the heads, each lane sixteen elements of a head.  A group stays with its token, so a lane's eight pairs of cos
-// and sin stay in registers.  N > 0: halves of the rotated part in pieces of N elements (the widest of 8, 4, 2 that divides rot / 2), of
-// which a lane holds both sides, so that a pair meets in a lane; kNeighbours: any pairs, in pieces of 8.
-constexpr int kNeighbours = 0;
-template <typename T, int N, bool NORM>
+// and sin stay in registers.  A lane's sixteen elements are pieces of BYTES, neighbouring lanes' pieces side by side.  kHalf: it holds both
+// sides of its pairs, pieces at q and at q + rot / 2 (BYTES: the most of 16, 8 and 4 that rot / 2 is a multiple of); kNeighbours: pairs
+// meet in a piece.  (8 consecutive fp32 a lane instead of 4: 4096 tokens of 40 heads of 128 30.6 us, now 28.5; fp16 in pieces of 2
+// bytes: 35.9 us, k_rope_any 25.7, but fp32 in pieces of 4 36.4, k_rope_any 42.1.)
+enum { kHalf = 0, kNeighbours = 1 };
+template <typename T, int MODE, int BYTES, bool NORM>
 __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
 {
-    constexpr int kPiece = N == kNeighbours ? 8 : N, kPairs = 8 / kPiece;   // elements of a piece; pairs of pieces of a lane
+    constexpr int kPiece = BYTES / sizeof(T), kPairs = 8 / kPiece;   // elements of a piece; pairs of pieces of a lane
+    // normalised fp16 neighbours: a lane's two pieces are one behind the other, which takes 72 registers instead of 80 (4096 tokens of
+    // 40 heads of 128 17.7 us, side by side 20.6; not normalised 16.1, side by side 14.7)
+    constexpr bool kTogether = MODE == kNeighbours && NORM && sizeof(T) == 2;
     __shared__ __align__(16) float2 table[kTable];
     pdl_trigger();
     pdl_wait();
     const int tid = threadIdx.x, heads = p.r[0].heads + p.r[1].heads;
     const int group = tid / p.lanes, lane = tid % p.lanes, groups_per_token = kThreads / p.lanes / p.tile;
     const int slot = group / groups_per_token, t0 = blockIdx.x * p.tile, t = t0 + slot;
-    // the pairs of pieces j * lanes + lane: first those that turn something, then what is passed on.  Offsets, -1 = none.
-    const int turning = N == kNeighbours ? (p.rot + 15) / 16 : p.half_rot / kPiece;
+    // offsets of the pieces, -1 = none.  kHalf: the pairs j * lanes + lane, first those that turn, then what is passed on
+    const int turning = p.half_rot / kPiece;
     int at[2][kPairs];
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) {
         const int q = j * p.lanes + lane;
-        if (q < turning) {
-            at[0][j] = N == kNeighbours ? 16 * q : kPiece * q;
-            at[1][j] = at[0][j] + (N == kNeighbours ? 8 : p.half_rot);
+        if (MODE == kNeighbours) {
+            at[0][j] = kTogether ? 2 * q * kPiece : q * kPiece;
+            at[1][j] = kTogether ? at[0][j] + kPiece : (q + kPairs * p.lanes) * kPiece;
+        } else if (q < turning) {
+            at[0][j] = q * kPiece;
+            at[1][j] = at[0][j] + p.half_rot;
         } else {
-            at[0][j] = (N == kNeighbours ? 16 * turning : p.rot) + 2 * kPiece * (q - turning);
+            at[0][j] = p.rot + 2 * kPiece * (q - turning);
             at[1][j] = at[0][j] + kPiece;
         }
         if (at[0][j] >= p.dim) at[0][j] = -1;
@@ -152,9 +164,9 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
     };
     const int step = groups_per_token * gridDim.y;
     int h = blockIdx.y * groups_per_token + group % groups_per_token;
-    // pieces of the next heads on their way while one is worked on: two heads of plain fp16 (8192 tokens of 40 heads of 128: 28.6 us,
-    // one: 30.2), one where there is a norm (35.1 us, two: 38.2) or fp32 (4096 tokens 32.6 us, two: 33.6)
-    constexpr int kAhead = NORM || sizeof(T) == 4 ? 1 : 2;
+    // pieces of the next heads on their way while one is worked on: two heads (8192 tokens of 40 heads of 128 fp16: 28.6 us, one:
+    // 30.2; 4096 fp32: 27.3 us, one: 28.7), one where there is a norm (35.1 us, two: 38.2)
+    constexpr int kAhead = NORM ? 1 : 2;
     struct Head {
         Piece<T, kPiece> in[2][kPairs];
         T* y;
@@ -183,12 +195,14 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
         if (t0 + s < p.tokens) table[i] = turn(p.positions[t0 + s], p.inv_freq[i - s * p.half_rot], p.factor);
     }
     __syncthreads();
-    float2 cs[8];   // of a lane's pairs; pairs that do not turn have none
+    // a lane's i-th pair, from half_rot on one that does not turn
+    auto pair_at = [&](int i) {
+        return kTogether ? 8 * lane + i : MODE == kNeighbours ? ((2 * i / kPiece * p.lanes + lane) * kPiece + 2 * i % kPiece) / 2 : (i / kPiece * p.lanes + lane) * kPiece + i % kPiece;
+    };
+    float2 cs[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int pair = (i / kPiece * p.lanes + lane) * kPiece + i % kPiece;
-        if (pair < p.half_rot) cs[i] = table[slot * p.half_rot + pair];
-    }
+    for (int i = 0; i < 8; ++i)
+        if (pair_at(i) < p.half_rot) cs[i] = table[slot * p.half_rot + pair_at(i)];
     auto work = [&](Head& now) {
         float v[16];   // first sides, second sides
         const bool live = t < p.tokens && h < heads;
@@ -228,8 +242,8 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (N == kNeighbours ? 8 * lane + i >= p.half_rot : i / kPiece * p.lanes + lane >= turning) continue;   // passed on
-            float &a = N == kNeighbours ? v[2 * i] : v[i], &b = N == kNeighbours ? v[2 * i + 1] : v[8 + i];
+            if (MODE == kNeighbours ? pair_at(i) >= p.half_rot : i / kPiece * p.lanes + lane >= turning) continue;   // passed on
+            float &a = MODE == kNeighbours ? v[2 * i] : v[i], &b = MODE == kNeighbours ? v[2 * i + 1] : v[8 + i];
             const float a0 = a, b0 = b;
             a = a0 * cs[i].x - b0 * cs[i].y;
             b = b0 * cs[i].x + a0 * cs[i].y;
@@ -256,8 +270,8 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
 
 // The same for any part, alignment and stride: a lane holds sixteen consecutive elements and finds the other element of a pair
 // in shared memory (pitch 17, so that lanes 16 elements apart meet different banks).  Its cos, signed sin and the places of the other
-// elements stay in registers.  Bound: the shared-memory traffic of 8 bytes an element.  4096 tokens of 40 heads of 128 fp16, 88 turned:
-// 27.1 us (k_rope with all 128 turned: 16.7); registers for 4 blocks an SM instead of 5: 31.5 us.
+// elements stay in registers.  Bound: the shared-memory traffic of 8 bytes an element.  4096 tokens of 40 heads of 128 fp16, 42 turned:
+// 25.8 us (k_rope, 44 turned: 18.9); with registers for 4 blocks an SM instead of 5 it was 31.5 us instead of 27.1.
 template <typename T, bool NORM>
 __global__ void __launch_bounds__(kThreads, 5) k_rope_any(const RopeParams p, bool wide)
 {
@@ -393,14 +407,15 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
 {
     const int heads = p.r[0].heads + p.r[1].heads;
     const bool wide = wide_rows(p, f32 ? 4 : 2) && p.dim % 8 == 0, norm = p.r[0].norm || p.r[1].norm;
-    // pieces of a half: the widest that divide it; neighbours meet in one piece whatever their number
-    const int piece = !wide ? 0 : p.interleaved || p.half_rot % 8 == 0 ? 8 : p.half_rot % 4 == 0 ? 4 : p.half_rot % 2 == 0 ? 2 : 0;
-    // lanes: pieces that turn, then what is passed on (of which kNeighbours leaves a piece of a lane empty at most)
+    // bytes of a piece: 16, or the most that half of what turns is a multiple of; 0: k_rope_any
+    const int size = f32 ? 4 : 2, half_bytes = p.half_rot * size;
+    const int bytes = !wide ? 0 : p.interleaved || half_bytes % 16 == 0 ? 16 : half_bytes % 8 == 0 ? 8 : half_bytes % 4 == 0 ? 4 : 0;
+    // lanes of a head: sixteen elements each, of halves both sides of what turns, then what is passed on
     int units = (p.dim + 15) / 16;
-    if (piece && p.interleaved) {
-        const int turning = (p.rot + 15) / 16;
-        units = turning + std::max(0, (p.dim - 16 * turning + 15) / 16);
-    } else if (piece == 8) units = p.half_rot / 8 + (p.dim - p.rot + 15) / 16;
+    if (bytes && !p.interleaved) {
+        const int piece = bytes / size, pairs = p.half_rot / piece + (p.dim - p.rot + 2 * piece - 1) / (2 * piece);
+        units = (pairs * piece + 7) / 8;
+    }
     p.lanes = 1;
     while (p.lanes < units) p.lanes *= 2;
     const int groups = kThreads / p.lanes;
@@ -422,19 +437,19 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     auto typed = [&](auto zero) {
         using T = decltype(zero);
         auto halves = [&](auto n) {
-            constexpr int N = decltype(n)::value;
-            norm ? go(k_rope<T, N, true>, "k_rope_half") : go(k_rope<T, N, false>, "k_rope_half");
+            constexpr int BYTES = decltype(n)::value;
+            norm ? go(k_rope<T, kHalf, BYTES, true>, "k_rope_half") : go(k_rope<T, kHalf, BYTES, false>, "k_rope_half");
         };
-        if (!piece) norm ? go(k_rope_any<T, true>, "k_rope_any", wide) : go(k_rope_any<T, false>, "k_rope_any", wide);
-        else if (p.interleaved) norm ? go(k_rope<T, kNeighbours, true>, "k_rope_neighbours") : go(k_rope<T, kNeighbours, false>, "k_rope_neighbours");
-        else if (piece == 8) halves(std::integral_constant<int, 8>{});
-        else if (piece == 4) halves(std::integral_constant<int, 4>{});
-        else halves(std::integral_constant<int, 2>{});
+        if (!bytes) norm ? go(k_rope_any<T, true>, "k_rope_any", wide) : go(k_rope_any<T, false>, "k_rope_any", wide);
+        else if (p.interleaved) norm ? go(k_rope<T, kNeighbours, 16, true>, "k_rope_neighbours") : go(k_rope<T, kNeighbours, 16, false>, "k_rope_neighbours");
+        else if (bytes == 16) halves(std::integral_constant<int, 16>{});
+        else if (bytes == 8) halves(std::integral_constant<int, 8>{});
+        else halves(std::integral_constant<int, 4>{});
     };
     if (f32) typed(0.0f);
     else typed(__half{});
     return describe(name, "<", f32 ? "float" : "half", norm ? ",norm" : "", "> block=", kThreads, " grid=", blocks_x, "x", blocks_y, " tokens=", p.tile,
-                    " lanes=", p.lanes, " piece=", piece);
+                    " lanes=", p.lanes, " piece=", bytes);
 }
 
 }  // namespace
