@@ -103,6 +103,27 @@ def test_rope_in_place(kind, D, rot, interleaved, norm):
     _check(x, pos, f, norms, interleaved, kinds=(kind, kind), in_place=True)
 
 
+@pytest.mark.parametrize("D,rot", [(80, 40), (128, 88), (256, 8), (80, 36), (128, 92), (512, 508), (80, 12), (80, 38), (128, 42), (24, 2), (8, 8), (16, 6)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+def test_rope_pieces(D, rot, interleaved, norm, dt):
+    """Every width of the pieces (16, 8, 4 bytes and none), by what half of the rotated part is a multiple of; what is passed on may be
+    infinite where no norm takes it in."""
+    x, pos, f, norms = _case(51, 53, 9, 2, D, rot, dt, norm)
+    if not norm and rot < D:
+        for t in x:
+            t[::3, :, rot] = float("inf")
+            t[1::3, 1:, D - 1] = float("-inf")
+    _check(x, pos, f, norms, interleaved, factor=0.75)
+    half = rot // 2 * x[0].element_size()
+    want = 16 if interleaved or half % 16 == 0 else 8 if half % 8 == 0 else 4 if half % 4 == 0 else 0
+    assert ops.last_launch().endswith(f" piece={want}") and ops.last_launch().startswith("k_rope_any") == (want == 0)
+    _check(x, pos, f, norms, interleaved, kinds=("gated", "packed"))
+    _check(x, pos, f, norms, interleaved, kinds=("shifted", "plain"))
+    _check(x, pos, f, norms, interleaved, kinds=("cache", "cache"), in_place=True)
+
+
 @pytest.mark.parametrize("dt", [torch.float16, torch.float32])
 def test_rope_far_and_negative_positions(dt):
     """Positions whose angle needs more than 32 bits, the largest and the most negative one."""
