@@ -96,22 +96,24 @@ template <int N> struct Piece<float, N> {
     }
 };
 // N of the norm's weights, bfloat16, at an offset of whole pieces.
-template <int N>
-__device__ __forceinline__ void norm_piece(float* x, const void* w, int at, float rinv, float bias)
-{
-    if constexpr (N == 1) {
-        x[0] = x[0] * rinv * (bf16_at(w, at) + bias);
-    } else {
-        using V = typename Piece<__half, N>::V;
-        const V v = *reinterpret_cast<const V*>(static_cast<const uint16_t*>(w) + at);
-        const uint32_t* h = reinterpret_cast<const uint32_t*>(&v);
+template <int N> struct Weights {
+    using V = typename std::conditional<N == 1, uint16_t, typename std::conditional<N == 2, uint32_t, typename std::conditional<N == 4, uint2, uint4>::type>::type>::type;
+    V v;
+    __device__ __forceinline__ void load(const void* w, int at) { v = *reinterpret_cast<const V*>(static_cast<const uint16_t*>(w) + at); }
+    __device__ __forceinline__ void scale(float* x, float rinv, float bias) const
+    {
+        if constexpr (N == 1) {
+            x[0] = x[0] * rinv * (__uint_as_float(uint32_t(v) << 16) + bias);
+        } else {
+            const uint32_t* h = reinterpret_cast<const uint32_t*>(&v);
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            x[2 * i] = x[2 * i] * rinv * (__uint_as_float(h[i] << 16) + bias);
-            x[2 * i + 1] = x[2 * i + 1] * rinv * (__uint_as_float(h[i] & 0xffff0000u) + bias);
+            for (int i = 0; i < N / 2; ++i) {
+                x[2 * i] = x[2 * i] * rinv * (__uint_as_float(h[i] << 16) + bias);
+                x[2 * i + 1] = x[2 * i + 1] * rinv * (__uint_as_float(h[i] & 0xffff0000u) + bias);
+            }
         }
     }
-}
+};
 
 constexpr int kThreads = 128, kTable = 2048;   // cos / sin pairs a block holds
 
@@ -122,13 +124,20 @@ constexpr int kThreads = 128, kTable = 2048;   // cos / sin pairs a block holds
 // meet in a piece.  (8 consecutive fp32 a lane instead of 4: 4096 tokens of 40 heads of 128 30.6 us, now 28.5; fp16 in pieces of 2
 // bytes: 35.9 us, k_rope_any 25.7, but fp32 in pieces of 4 36.4, k_rope_any 42.1.)
 enum { kHalf = 0, kNeighbours = 1 };
-template <typename T, int MODE, int BYTES, bool NORM>
-__global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
+// NORM kEarly: the norm's weights are on their way during the sum of squares, for grids whose blocks all run at once with the registers
+// that it takes (421 tokens of 28 heads of 256 4.8 us, kNorm 5.6; 8192 of 40 of 128, more than run at once, 41 us, kNorm 34).
+enum { kPlain = 0, kNorm = 1, kEarly = 2 };
+constexpr int early_blocks(int size, int bytes) { return size == 2 && bytes == 16 ? 6 : 5; }   // of an SM
+// Blocks of an SM that the registers have to allow (normalised fp16 neighbours left to themselves take 80: 4096 tokens of 40 heads of 128
+// 20.8 us, now 18.0).
+constexpr int min_blocks(int size, int mode, int bytes, int norm) { return norm == kEarly ? early_blocks(size, bytes) : norm == kNorm && mode == kNeighbours && size == 2 ? 7 : 1; }
+template <typename T, int MODE, int BYTES, int NORM>
+__global__ void __launch_bounds__(kThreads, min_blocks(sizeof(T), MODE, BYTES, NORM)) k_rope(const RopeParams p)
 {
     constexpr int kPiece = BYTES / sizeof(T), kPairs = 8 / kPiece;   // elements of a piece; pairs of pieces of a lane
     // normalised fp16 neighbours: a lane's two pieces are one behind the other, which takes 72 registers instead of 80 (4096 tokens of
-    // 40 heads of 128 17.7 us, side by side 20.6; not normalised 16.1, side by side 14.7)
-    constexpr bool kTogether = MODE == kNeighbours && NORM && sizeof(T) == 2;
+    // 40 heads of 128 18.0 us, side by side 20.6; not normalised 16.1, side by side 14.7)
+    constexpr bool kTogether = MODE == kNeighbours && NORM != kPlain && sizeof(T) == 2;
     __shared__ __align__(16) float2 table[kTable];
     pdl_trigger();
     pdl_wait();
@@ -166,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
     int h = blockIdx.y * groups_per_token + group % groups_per_token;
     // pieces of the next heads on their way while one is worked on: two heads (8192 tokens of 40 heads of 128 fp16: 28.6 us, one:
     // 30.2; 4096 fp32: 27.3 us, one: 28.7), one where there is a norm (35.1 us, two: 38.2)
-    constexpr int kAhead = NORM ? 1 : 2;
+    constexpr int kAhead = NORM != kPlain ? 1 : 2;
     struct Head {
         Piece<T, kPiece> in[2][kPairs];
         T* y;
@@ -226,7 +235,15 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
                 }
         fetch(now, h + kAhead * step);
         h += step;
-        if constexpr (NORM) {
+        if constexpr (NORM != kPlain) {
+            Weights<kPiece> weights[2][kPairs];
+            if (NORM == kEarly && live && w) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < kPairs; ++j)
+                        if (at[i][j] >= 0) weights[i][j].load(w, at[i][j]);
+            }
             float s = 0.f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) s = fmaf(v[j], v[j], s);
@@ -237,7 +254,10 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int j = 0; j < kPairs; ++j)
-                        if (at[i][j] >= 0) norm_piece<kPiece>(v + 8 * i + kPiece * j, w, at[i][j], rinv, p.bias);
+                        if (at[i][j] >= 0) {
+                            if (NORM != kEarly) weights[i][j].load(w, at[i][j]);
+                            weights[i][j].scale(v + 8 * i + kPiece * j, rinv, p.bias);
+                        }
             }
         }
 #pragma unroll
@@ -266,7 +286,7 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeParams p)
 }
 
 // Bound: HBM.  8192 tokens of 40 heads of 128 fp16: 28.6 us (5.9 TB/s; with 256 threads a block 31.8), normalised 33.8; 421 tokens of 28
-// heads of 256, a quarter turned, normalised: 5.5 us.
+// heads of 256, a quarter turned, normalised: 4.8 us.
 
 // The same for any part, alignment and stride: a lane holds sixteen consecutive elements and finds the other element of a pair
 // in shared memory (pitch 17, so that lanes 16 elements apart meet different banks).  Its cos, signed sin and the places of the other
@@ -330,8 +350,11 @@ __global__ void __launch_bounds__(kThreads, 5) k_rope_any(const RopeParams p, bo
             if (live && r.norm) {
                 const float rinv = rsqrtf(s / float(p.dim) + p.eps);
                 if (wide && e0 + 16 <= p.dim) {
-                    norm_piece<8>(v, r.norm, e0, rinv, p.bias);
-                    norm_piece<8>(v + 8, r.norm, e0 + 8, rinv, p.bias);
+                    Weights<8> a, b;
+                    a.load(r.norm, e0);
+                    b.load(r.norm, e0 + 8);
+                    a.scale(v, rinv, p.bias);
+                    b.scale(v + 8, rinv, p.bias);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -436,15 +459,17 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     };
     auto typed = [&](auto zero) {
         using T = decltype(zero);
-        auto halves = [&](auto n) {
-            constexpr int BYTES = decltype(n)::value;
-            norm ? go(k_rope<T, kHalf, BYTES, true>, "k_rope_half") : go(k_rope<T, kHalf, BYTES, false>, "k_rope_half");
+        const bool early = blocks_x * blocks_y <= 148 * early_blocks(size, bytes);
+        auto pieces = [&](auto mode, auto n, const char* what) {
+            constexpr int MODE = decltype(mode)::value, BYTES = decltype(n)::value;
+            !norm ? go(k_rope<T, MODE, BYTES, kPlain>, what) : early ? go(k_rope<T, MODE, BYTES, kEarly>, what) : go(k_rope<T, MODE, BYTES, kNorm>, what);
         };
+        const std::integral_constant<int, kHalf> halves;
         if (!bytes) norm ? go(k_rope_any<T, true>, "k_rope_any", wide) : go(k_rope_any<T, false>, "k_rope_any", wide);
-        else if (p.interleaved) norm ? go(k_rope<T, kNeighbours, 16, true>, "k_rope_neighbours") : go(k_rope<T, kNeighbours, 16, false>, "k_rope_neighbours");
-        else if (bytes == 16) halves(std::integral_constant<int, 16>{});
-        else if (bytes == 8) halves(std::integral_constant<int, 8>{});
-        else halves(std::integral_constant<int, 4>{});
+        else if (p.interleaved) pieces(std::integral_constant<int, kNeighbours>{}, std::integral_constant<int, 16>{}, "k_rope_neighbours");
+        else if (bytes == 16) pieces(halves, std::integral_constant<int, 16>{}, "k_rope_half");
+        else if (bytes == 8) pieces(halves, std::integral_constant<int, 8>{}, "k_rope_half");
+        else pieces(halves, std::integral_constant<int, 4>{}, "k_rope_half");
     };
     if (f32) typed(0.0f);
     else typed(__half{});
