@@ -452,6 +452,7 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     int blocks_y = 1;
     while (blocks_x * blocks_y < 148 * 4 && blocks_y * groups / p.tile < heads) ++blocks_y;
     const dim3 grid(blocks_x, blocks_y);
+    const bool early = norm && bytes && blocks_x * blocks_y <= 148 * early_blocks(size, bytes);
     const char* name = "";
     auto go = [&](auto kern, const char* what, auto... more) {
         launch_pdl(kern, grid, dim3(kThreads), 0, st, "rope launch", p, more...);
@@ -459,7 +460,6 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     };
     auto typed = [&](auto zero) {
         using T = decltype(zero);
-        const bool early = blocks_x * blocks_y <= 148 * early_blocks(size, bytes);
         auto pieces = [&](auto mode, auto n, const char* what) {
             constexpr int MODE = decltype(mode)::value, BYTES = decltype(n)::value;
             !norm ? go(k_rope<T, MODE, BYTES, kPlain>, what) : early ? go(k_rope<T, MODE, BYTES, kEarly>, what) : go(k_rope<T, MODE, BYTES, kNorm>, what);
@@ -473,7 +473,7 @@ std::string launch_rope(RopeParams p, bool f32, cudaStream_t st)
     };
     if (f32) typed(0.0f);
     else typed(__half{});
-    return describe(name, "<", f32 ? "float" : "half", norm ? ",norm" : "", "> block=", kThreads, " grid=", blocks_x, "x", blocks_y, " tokens=", p.tile,
+    return describe(name, "<", f32 ? "float" : "half", early ? ",norm early" : norm ? ",norm" : "", "> block=", kThreads, " grid=", blocks_x, "x", blocks_y, " tokens=", p.tile,
                     " lanes=", p.lanes, " piece=", bytes);
 }
 

@@ -124,6 +124,17 @@ def test_rope_pieces(D, rot, interleaved, norm, dt):
     _check(x, pos, f, norms, interleaved, kinds=("cache", "cache"), in_place=True)
 
 
+@pytest.mark.parametrize("T,early", [(4001, False), (500, True)])
+@pytest.mark.parametrize("D,rot,interleaved", [(128, 128, False), (80, 40, False), (128, 92, False), (80, 38, False), (96, 90, True)])
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+def test_rope_norms_of_few_and_many_blocks(T, early, D, rot, interleaved, dt):
+    """The two ways to read the norm's weights."""
+    x, pos, f, norms = _case(T + rot, T, 6, 1, D, rot, dt, True)
+    _check(x, pos, f, norms, interleaved)
+    assert ("early" in ops.last_launch()) == (early and "any" not in ops.last_launch())
+    _check(x, pos, f, [norms[0], None], interleaved, kinds=("packed", "gated"))
+
+
 @pytest.mark.parametrize("dt", [torch.float16, torch.float32])
 def test_rope_far_and_negative_positions(dt):
     """Positions whose angle needs more than 32 bits, the largest and the most negative one."""
