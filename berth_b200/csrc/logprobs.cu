@@ -93,7 +93,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 struct Part {
     float m, z, t;
 };
-__device__ __forceinline__ float redux_max(float v) { float r; asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float redux_max(float v) { float r; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 // p, whose maximum is not the one that keeps its 1 out of the sum, relative to the maximum m.
 __device__ __forceinline__ Part beside(Part p, float m, float scale2)
