@@ -132,6 +132,15 @@ static int to_int(PyObject* o, const char* what, const char* name)
 }
 static void* to_stream(PyObject* o) { return o == Py_None ? NULL : PyLong_AsVoidPtr(o); }
 
+/* The library's call without the interpreter's lock: a launch waits where the device's queue is full or its code is still to be loaded,
+ * and what the stream waits for may be a peer whose thread needs the lock. */
+#define UNLOCKED(rc, call)         \
+    do {                           \
+        Py_BEGIN_ALLOW_THREADS     \
+        rc = (call);               \
+        Py_END_ALLOW_THREADS       \
+    } while (0)
+
 static PyObject* answer(int rc, const char* what, const char* (*last)(void))
 {
     if (rc == 0) Py_RETURN_NONE;
@@ -203,9 +212,10 @@ static PyObject* py_rope(PyObject* self, PyObject* const* a, Py_ssize_t n)
     const double factor = PyFloat_AsDouble(a[7]), eps = PyFloat_AsDouble(a[10]), bias = PyFloat_AsDouble(a[11]);
     void* stream = to_stream(a[12]);
     if (interleaved < 0 || PyErr_Occurred()) return NULL;
-    return answer(berth_ops_rope(&rq, has_k ? &rk : NULL, pos.ptr, freq.ptr, (int) q[0].shape[0], (int) q[0].shape[2], 2 * (int) freq.shape[0], interleaved,
-                                 (float) factor, (float) eps, (float) bias, f32, stream),
-                  "rope", berth_ops_last_error);
+    int rc;
+    UNLOCKED(rc, berth_ops_rope(&rq, has_k ? &rk : NULL, pos.ptr, freq.ptr, (int) q[0].shape[0], (int) q[0].shape[2], 2 * (int) freq.shape[0], interleaved,
+                                (float) factor, (float) eps, (float) bias, f32, stream));
+    return answer(rc, "rope", berth_ops_last_error);
 }
 
 /* logprobs(logits, tokens, logprob, rank, entropy, top_idx, top_logprob, vocab or None, inv_temp, stream) */
@@ -252,10 +262,11 @@ static PyObject* py_logprobs(PyObject* self, PyObject* const* a, Py_ssize_t n)
     const double inv_temp = PyFloat_AsDouble(a[8]);
     void* stream = to_stream(a[9]);
     if (PyErr_Occurred()) return NULL;
-    return answer(berth_ops_logprobs(x.ptr, f32, x.stride[0], token.given ? token.ptr : NULL, (float) inv_temp, lp.given ? lp.ptr : NULL,
-                                     rank.given ? rank.ptr : NULL, entropy.given ? entropy.ptr : NULL, best ? top.ptr : NULL, best ? top_lp.ptr : NULL,
-                                     (int) best, (int) rows, vocab, stream),
-                  what, berth_ops_last_error);
+    int rc;
+    UNLOCKED(rc, berth_ops_logprobs(x.ptr, f32, x.stride[0], token.given ? token.ptr : NULL, (float) inv_temp, lp.given ? lp.ptr : NULL,
+                                    rank.given ? rank.ptr : NULL, entropy.given ? entropy.ptr : NULL, best ? top.ptr : NULL, best ? top_lp.ptr : NULL,
+                                    (int) best, (int) rows, vocab, stream));
+    return answer(rc, what, berth_ops_last_error);
 }
 
 /* route(logits, selection_bias, topk_idx, topk_w, top_k, score, n_group, topk_group, group_score, renormalize, scale, stream) */
@@ -283,9 +294,10 @@ static PyObject* py_route(PyObject* self, PyObject* const* a, Py_ssize_t n)
         return NULL;
     const tensor* ts[4] = {&x, &bias, &idx, &w};
     if (same_device(what, ts, 4)) return NULL;
-    return answer(berth_moe_route(x.ptr, f32, x.stride[0], bias.given ? bias.ptr : NULL, idx.given ? idx.ptr : NULL, w.given ? w.ptr : NULL, (int) rows,
-                                  (int) experts, k, score, groups, kept, group_score, renormalize, (float) scale, stream),
-                  what, berth_moe_last_error);
+    int rc;
+    UNLOCKED(rc, berth_moe_route(x.ptr, f32, x.stride[0], bias.given ? bias.ptr : NULL, idx.given ? idx.ptr : NULL, w.given ? w.ptr : NULL, (int) rows,
+                                 (int) experts, k, score, groups, kept, group_score, renormalize, (float) scale, stream));
+    return answer(rc, what, berth_moe_last_error);
 }
 
 /* init(Error, torch.Tensor): the exception to raise and the class of the tensors */
