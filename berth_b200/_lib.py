@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import subprocess
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.path.join(_HERE, "libberth_b200.so")
@@ -160,9 +161,9 @@ _lib = None
 
 
 def build(verbose: bool = False) -> str:
-    """Compile the CUDA library in-tree with the Makefile under csrc/ (nvcc, sm_100a)."""
+    """Compile the CUDA library in-tree with the Makefile under csrc/ (nvcc, sm_100a), and the callers of this interpreter."""
     out = None if verbose else subprocess.DEVNULL
-    subprocess.run(["make", "-C", CSRC, "-j8"], check=True, stdout=out)
+    subprocess.run(["make", "-C", CSRC, "-j8", "bind", f"PYTHON={sys.executable}"], check=True, stdout=out)
     return SO_PATH
 
 
@@ -179,7 +180,8 @@ def bind():
         try:
             from . import _bind as module
         except ImportError as exc:
-            raise RuntimeError(f"berth_b200/_bind.so cannot be loaded ({exc}): build it with `make -C {CSRC}`") from exc
+            raise RuntimeError(f"berth_b200's compiled callers cannot be loaded ({exc}): build them with "
+                               f"`make -C {CSRC} bind PYTHON={sys.executable}`") from exc
         module.init(Error, torch.Tensor)
         _bind = module
     return _bind
