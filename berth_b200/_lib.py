@@ -171,7 +171,8 @@ _bind = None
 
 
 def bind():
-    """The compiled callers of the operators that read torch tensors (csrc/bind.c).  Raises if they have not been built."""
+    """The compiled callers of the operators that read torch tensors (csrc/bind.c).  Raises if they have not been built, or
+    for a torch that does not publish what they read tensors through (2.11 does)."""
     global _bind
     if _bind is None:
         lib()

@@ -300,6 +300,7 @@ static PyObject* py_route(PyObject* self, PyObject* const* a, Py_ssize_t n)
     return answer(rc, what, berth_moe_last_error);
 }
 
+#define NEEDS "rope, logprobs and route read tensors through: torch 2.11 publishes it"
 /* init(Error, torch.Tensor): the exception to raise and the class of the tensors */
 static PyObject* py_init(PyObject* self, PyObject* const* a, Py_ssize_t n)
 {
@@ -309,12 +310,19 @@ static PyObject* py_init(PyObject* self, PyObject* const* a, Py_ssize_t n)
         return NULL;
     }
     PyObject* capsule = PyObject_GetAttrString(a[1], "__dlpack_c_exchange_api__");
-    if (!capsule) return NULL;
+    if (!capsule) {
+        if (PyErr_ExceptionMatches(PyExc_AttributeError)) {
+            PyErr_Clear();
+            PyErr_Format(PyExc_ImportError, "%s has no __dlpack_c_exchange_api__ (DLPack 1.x), which " NEEDS, ((PyTypeObject*) a[1])->tp_name);
+        }
+        return NULL;
+    }
     const dl_exchange* x = (const dl_exchange*) PyCapsule_GetPointer(capsule, "dlpack_exchange_api");   /* lives as long as torch */
     Py_DECREF(capsule);
     if (!x) return NULL;
     if (x->version.major != 1 || !x->tensor_from_object) {
-        PyErr_SetString(PyExc_ImportError, "torch.Tensor offers no DLPack 1.x exchange interface");
+        PyErr_Format(PyExc_ImportError, "%s offers an exchange interface of DLPack %d.%d; version 1.x " NEEDS, ((PyTypeObject*) a[1])->tp_name,
+                     (int) x->version.major, (int) x->version.minor);
         return NULL;
     }
     g_exchange = x;

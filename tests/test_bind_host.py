@@ -150,3 +150,29 @@ def test_two_threads_launch_side_by_side(stubbed, name):
     run = _start(stubbed, name, 2)
     assert run(1) == ([None, None], 2)
     assert run(-1) == (["not let", "not let"], 2)
+
+
+def test_a_torch_without_the_exchange_interface_is_named(stubbed, monkeypatch):
+    """init() and the package's bind() say which interface is missing, in which torch, and which torch has it; init() keeps what it has."""
+    module, _ = stubbed
+
+    class Bare:
+        pass
+    with pytest.raises(ImportError, match="__dlpack_c_exchange_api__.*torch 2.11"):
+        module.init(Refused, Bare)
+    old = DlExchange(0, 9, None, None, None, None, C.cast(_read, C.c_void_p), None)
+
+    class Other:
+        __dlpack_c_exchange_api__ = _capsule_new(C.addressof(old), C.cast(_name, C.c_char_p), None)
+    with pytest.raises(ImportError, match="DLPack 0.9.*torch 2.11"):
+        module.init(Refused, Other)
+    with pytest.raises(Refused, match="must be a torch tensor"):      # still those of the first init
+        module.route(Bare(), *[None] * 11)
+
+    import torch
+    from berth_b200 import _lib
+    monkeypatch.setattr(_lib, "_bind", None)
+    monkeypatch.setattr(torch, "Tensor", Bare)
+    with pytest.raises(ImportError, match="__dlpack_c_exchange_api__"):
+        _lib.bind()
+    assert _lib._bind is None
