@@ -532,7 +532,8 @@ extern "C" int berth_ops_rope_frequencies(double* inv_freq, int rot_dim, double 
             auto pair_of = [&](double turns) { return rot_dim * std::log(scaling->original_context / (turns * two_pi)) / (2.0 * std::log(base)); };
             lo = std::max(std::floor(pair_of(scaling->beta_fast)), 0.0);
             hi = std::min(std::ceil(pair_of(scaling->beta_slow)), rot_dim - 1.0);
-            if (hi - lo < 1e-3) hi = lo + 1e-3;
+            if (pair_of(scaling->beta_slow) <= 0.0 && pair_of(scaling->beta_fast) < 0.0) lo = -1.0, hi = 0.0;   // not even pair 0 turns more than beta_slow times
+            else if (hi - lo < 1e-3) hi = lo + 1e-3;
         }
         if (kind == 4 && !(scaling->low_factor > 0.0 && scaling->high_factor > scaling->low_factor && std::isfinite(scaling->high_factor)))
             throw std::runtime_error("rope frequencies: high_factor must be finite and above low_factor, which must be positive");

@@ -279,8 +279,9 @@ int berth_ops_rope(const berth_rope_rows* q, const berth_rope_rows* k, const int
  * longer than the trained one.  scaling NULL or kind 0: unscaled.  kind 1: every frequency divided by factor.  kind 2:
  * base * factor^(rot_dim / (rot_dim - 2)) in the place of base (rot_dim > 2).  kind 3: frequencies that turn at least
  * beta_fast times within original_context are kept, those of at most beta_slow turns divided by factor, a linear blend
- * over the pair index between the two (bounds rounded outwards to whole pairs), and *attention_factor =
- * 0.1 ln(factor) + 1 unless attention_factor_override > 0.  kind 4: kept above high_factor turns, divided by factor below low_factor turns,
+ * over the pair index between the two (bounds rounded outwards to whole pairs, then brought into 0 .. rot_dim - 1; a
+ * context in which no pair turns more than beta_slow times: all divided), and *attention_factor = 0.1 ln(factor) + 1
+ * unless attention_factor_override > 0.  kind 4: kept above high_factor turns, divided by factor below low_factor turns,
  * in between blended by (turns - low_factor) / (high_factor - low_factor).  *attention_factor (may be NULL) is 1 for the
  * other kinds.  -1 and berth_ops_last_error for values out of range. */
 typedef struct berth_rope_scaling {

@@ -219,3 +219,28 @@ def test_rope_refuses_outputs_whose_heads_overlap(lib, yt, yh):
     q = _rows(x=2 * P, yt=yt, yh=yh)
     assert lib.berth_ops_rope(q, None, P, P, 3, 64, 64, 0, 1.0, 1e-6, 0.0, 0, None) == -1
     assert "overlap" in ops.last_error()
+
+
+# ------------------------------------------------------------------ frequencies: ends of the ranges
+
+@pytest.mark.parametrize("ctx,fast,slow", [(1.0, 32.0, 1.0), (4.0, 32.0, 1.0), (6.0, 1.0, 1.0), (100.0, 64.0, 32.0), (100.0, 16.0, 16.0)])
+@pytest.mark.parametrize("rot", [2, 64])
+def test_yarn_divides_every_pair_of_a_context_too_short_for_any(rot, ctx, fast, slow):
+    """ctx / (2 pi) turns of the fastest pair: at most beta_slow, so that every frequency is divided by the factor."""
+    assert ctx / (2 * math.pi) < slow
+    f, _ = ops.rope_frequencies(rot, 1e4, "yarn", factor=4.0, original_context=ctx, beta_fast=fast, beta_slow=slow)
+    _steps(f, [1e4 ** (-2.0 * i / rot) / 4.0 for i in range(rot // 2)], 4)
+
+
+@pytest.mark.parametrize("ctx,fast,slow", [(1e12, 32.0, 1.0), (2000.0, 2.0, 1e-9), (7.0, 1.0, 1.0), (50.0, 32.0, 1.0)])
+def test_yarn_at_the_ends_of_the_pairs(ctx, fast, slow):
+    """Bounds outside of the pairs: the formula with both brought into 0 .. rot_dim - 1; a pair of beta_fast turns or more is as it was."""
+    rot, base, factor = 64, 1e4, 8.0
+    f, _ = ops.rope_frequencies(rot, base, "yarn", factor=factor, original_context=ctx, beta_fast=fast, beta_slow=slow)
+    plain = np.array([base ** (-2.0 * i / rot) for i in range(rot // 2)])
+    turns = ctx * plain / (2 * math.pi)
+    assert (np.array(f)[turns >= fast] == plain[turns >= fast]).all()
+    lo = max(math.floor(rot * math.log(ctx / (fast * 2 * math.pi)) / (2 * math.log(base))), 0)
+    hi = min(math.ceil(rot * math.log(ctx / (slow * 2 * math.pi)) / (2 * math.log(base))), rot - 1)
+    ramp = np.clip((np.arange(rot // 2) - lo) / (hi - lo), 0, 1) if hi > lo else (np.arange(rot // 2) > lo) * 1.0
+    _steps(f, plain * (1 - ramp) + plain / factor * ramp, 8)
