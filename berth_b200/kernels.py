@@ -349,7 +349,9 @@ class ops:
         import ctypes as C
         if scaling not in ops.ROPE_SCALING:
             raise Error(f"rope frequencies: scaling must be one of {', '.join(ops.ROPE_SCALING)}, got {scaling!r}")
-        out, af = (C.c_double * max(1, rot_dim // 2))(), C.c_float()
+        if not 2 <= rot_dim <= 512:   # (ctypes would cut a larger number to a C int)
+            raise Error(f"rope frequencies: rot_dim must be positive, even and at most 512, got {rot_dim}")
+        out, af = (C.c_double * (rot_dim // 2))(), C.c_float()
         sc = _lib.RopeScaling(ops.ROPE_SCALING[scaling], factor, original_context, beta_fast, beta_slow, low_factor, high_factor, attention_factor)
         if _lib.lib().berth_ops_rope_frequencies(out, rot_dim, base, C.byref(sc), C.byref(af)) != 0:
             raise Error(ops.last_error())

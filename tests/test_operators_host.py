@@ -244,3 +244,10 @@ def test_yarn_at_the_ends_of_the_pairs(ctx, fast, slow):
     hi = min(math.ceil(rot * math.log(ctx / (slow * 2 * math.pi)) / (2 * math.log(base))), rot - 1)
     ramp = np.clip((np.arange(rot // 2) - lo) / (hi - lo), 0, 1) if hi > lo else (np.arange(rot // 2) > lo) * 1.0
     _steps(f, plain * (1 - ramp) + plain / factor * ramp, 8)
+
+
+@pytest.mark.parametrize("rot", [2**32 + 64, -2**32 + 64, 2**31, 10**15, -2, 1 << 40])
+def test_frequencies_refuse_a_rot_dim_past_the_c_type(rot):
+    """Refused as it is, not as what a C int makes of it, and before a table of that size is asked for."""
+    with pytest.raises(Error, match="rot_dim"):
+        ops.rope_frequencies(rot, 1e4)
