@@ -522,6 +522,7 @@ extern "C" int berth_ops_rope_frequencies(double* inv_freq, int rot_dim, double 
         if (kind == 2) {
             if (rot_dim < 4) throw std::runtime_error("rope frequencies: a scaled base needs rot_dim of at least 4");
             base *= std::pow(f, double(rot_dim) / (rot_dim - 2));
+            if (!std::isfinite(base)) throw std::runtime_error("rope frequencies: the scaled base is out of range");
         }
         if (kind >= 3 && !(std::isfinite(scaling->original_context) && scaling->original_context >= 1.0))
             throw std::runtime_error("rope frequencies: original_context must be finite and at least 1");

@@ -251,3 +251,10 @@ def test_frequencies_refuse_a_rot_dim_past_the_c_type(rot):
     """Refused as it is, not as what a C int makes of it, and before a table of that size is asked for."""
     with pytest.raises(Error, match="rot_dim"):
         ops.rope_frequencies(rot, 1e4)
+
+
+def test_frequencies_refuse_a_scaled_base_past_the_type():
+    """base * factor^(rot_dim / (rot_dim - 2)) above the largest double would leave frequencies of zero."""
+    with pytest.raises(Error, match="scaled base"):
+        ops.rope_frequencies(64, 1e4, "ntk", factor=1e300)
+    assert min(ops.rope_frequencies(64, 1e4, "ntk", factor=1e280)[0]) > 0
