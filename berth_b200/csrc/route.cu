@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
             if (i < cnt) {
                 lo = fminf(lo, b);
                 hi = fmaxf(hi, b);
-                odd |= !(fabsf(b) < 1e30f);
+                odd |= !(fabsf(b) < 67108864.f);
             }
         }
         low = redux_min(lo);
@@ -332,7 +332,9 @@ __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteP
 #pragma unroll
             for (int i = 0; i < PER; ++i) bias[i] -= low;   // scores from 0 on: the order is the same
         }
-        if (__any_sync(dq::kFull, odd)) span = INFINITY;   // every row in 64 bits
+        // every row in 64 bits where the sum's rounding there, 2^-53 of the bias, is not small beside a step of the keys: sums that are
+        // equal in 64 bits are ties, which the scores less the common bias are not
+        if (__any_sync(dq::kFull, odd)) span = INFINITY;
     } else if constexpr (kHeldBias) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) bias[i] = 0.f;

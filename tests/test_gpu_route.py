@@ -290,3 +290,15 @@ def test_route_refuses_tensors_that_do_not_fit():
         args.update(bad)
         with pytest.raises(Error):
             moe.route(**args)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,keep,gs", [(1, 1, "max"), (8, 3, "top2"), (8, 3, "max")])
+@pytest.mark.parametrize("size", [2.0**25, 2.0**27, -2.0**33, 1e10, -1e12, 1e20, 3e38])
+def test_biases_that_swallow_the_scores(score, groups, keep, gs, size):
+    """A bias of which 64 bits leave few or none of a score's: choice scores that are equal there are ties, for the lower expert.  One
+    bias for all, two sizes, and the large one for every other expert (a mask by bias)."""
+    T, E, k = 24, 256, 8
+    l, b = _make(31, T, E)
+    for bias in (np.full(E, size), size * (1 + np.arange(E) // 64 % 2 * 2.0**-20), np.where(np.arange(E) % 2, size, b)):
+        _check(l, bias.astype(np.float32), k, score=score, groups=groups, keep=keep, group_score=gs)
