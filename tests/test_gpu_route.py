@@ -302,3 +302,30 @@ def test_biases_that_swallow_the_scores(score, groups, keep, gs, size):
     l, b = _make(31, T, E)
     for bias in (np.full(E, size), size * (1 + np.arange(E) // 64 % 2 * 2.0**-20), np.where(np.arange(E) % 2, size, b)):
         _check(l, bias.astype(np.float32), k, score=score, groups=groups, keep=keep, group_score=gs)
+
+
+@pytest.mark.parametrize("rank", [0, 1])
+def test_stages_of_one_rank_choose_among_all_ranks_experts(oracle, rank):
+    """GpuStages that hold half of the layer's experts: the bias and the groups are those of all of them."""
+    H, I, E, k, T = 256, 128, 32, 4, 24
+    wts = synth.moe_layer_weights(1234, "rt", H, I, E, k, 4, 2, shared_inter=128)
+    bias = np.random.default_rng(6).normal(0, 0.1, E).astype(np.float32)
+    x = synth.activations(1234, "rt.half", T, H)
+    half = {**wts, "n_experts": E // 2}
+    for name in ("gate", "up", "down"):
+        for part in ("trellis", "suh", "svh"):
+            half[f"{name}_{part}"] = wts[f"{name}_{part}"][rank * E // 2:(rank + 1) * E // 2]
+    device = torch.device("cuda", torch.cuda.current_device())
+    for r in ROUTINGS:
+        want_idx, want_w = _want(oracle, wts, x, r, bias)
+        assert (want_idx < E // 2).any() and (want_idx >= E // 2).any()
+        st = moe.GpuStages(device, half, E, max_rows=T * k + T, max_rows_per_expert=T, routing=moe.Routing(selection_bias=bias, **r))
+        xd = dev(x)
+        idx, w, inv, rows, counts = st.ep_send(xd, T)
+        torch.cuda.synchronize()
+        for i, v in ((idx, w), st.route(xd)):
+            assert (i.cpu().numpy() == want_idx).all()
+            assert np.allclose(v.cpu().numpy(), want_w, rtol=80 * 2.0 ** -24, atol=0)
+        assert (counts.cpu().numpy() == np.bincount(want_idx.ravel(), minlength=E)).all()
+        assert torch.equal(rows[inv.long()].view(torch.int16), xd.repeat_interleave(k, 0).view(torch.int16))
+    assert kernels.device_status(torch.cuda.current_device()) == 0
