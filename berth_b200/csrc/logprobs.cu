@@ -4,7 +4,8 @@
 // z = sum 2^y and t = sum 2^y y, y = (x - M) * inv_temp * log2 e: ln p = (x - m) * inv_temp - ln z and the entropy
 // ln z - t / z * ln 2 follow from the joined (m, z, t).  A thread adds its vectors' sums, trees of 16 or 32, with the rounding
 // kept aside, and joins carry z less the maximum's own 1: a certain row has z = 1 + little, and its entropy is made of that
-// little.  The rank of a given token is a count of the logits before it, taken in the same walk.
+// little.  (The logits of the maximum's own step, 15 fp32 or 31 fp16, meet its 1 in their tree: up to five roundings of 2^-24, an error
+// of 3e-7 in ln p and entropy.)  The rank of a given token is a count of the logits before it, taken in the same walk.
 //
 // The n best come out of the walk's by-product, the threads' maxima.  The cluster's warps fall into 32 or 64 groups (or give their k
 // largest threads each, where there are fewer warps): as many different logits that the row reaches.  At least n logits reach the
@@ -295,10 +296,13 @@ __device__ __noinline__ void sorted_lists(Shared<WARPS>& sh, const char* row, co
 // Vector i of the row belongs to thread i % kThreads of CTA (i / kThreads) % ctas, so that every warp sees all of the
 // vocabulary: a threshold taken from the warps' maxima then holds where the likely tokens lie close together.  The walk takes 4
 // vectors of a thread at a time, while those of the next step are on their way to shared memory.
-// Bound: long rows, instructions (9.2 warp instructions per 32 logits, 70 % of the issue slots) and ex2 (67 % of its pipe) before
-// HBM; few rows, the fixed parts of a call (cluster barriers, the dependent reads of the candidates, the join: 4 to 5 us).
-// 421 x 248320 fp16, 5 alternatives, 47.5 us (4.4 TB/s), without alternatives 42.1; 32 x 248320 fp32 12.0 us (2.6 TB/s); 77 x 100003 fp32
-// 9.4 us (3.3 TB/s); 1 x 248320 fp32 8.2 us.
+// Bound: long rows, instructions (9.9 warp instructions per 32 logits, 67 % of the issue slots) and ex2 (62 % of its pipe) before
+// HBM; few rows, the fixed parts of a call (cluster barriers, the dependent reads of the candidates, the join: 4 to 5 us); rows with
+// fewer finite logits than alternatives, the scan with sorted lists.
+// Inputs that change from call to call: 421 x 248320 fp16, 5 alternatives, 52.4 us (4.0 TB/s), without alternatives 5.5 less; 32 x 248320
+// fp32 12.0 us (2.7 TB/s), of which three logits are finite 32; 77 x 100003 fp32 9.1 us (3.4 TB/s); 1 x 248320 fp32, 20 alternatives, 7.9
+// us, of which ten are finite 26.  (Variants are compared, here and below, by calls on the same buffers, part of which the L2 holds: the
+// first takes 47.5 there.)
 template <bool F32, bool RANK, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_logprobs(const LogprobParams p)
 {

@@ -199,3 +199,32 @@ def test_two_threads_on_streams_of_their_own():
     assert all(isinstance(s, str) and s.startswith("k_logprobs") for s in said), said
     for a, b in zip(want, got):
         assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("V", [40, 3001, 100003])
+def test_log_probabilities_of_certain_rows(V, f32):
+    """Rows whose largest logit holds all but 10^-4 to 10^-16: ln p and entropy are small numbers, off by at most the roundings at the
+    maximum's 1 in its own step (five levels of a tree, half a step of 2^-23 each) and by their own relative errors."""
+    r = np.random.default_rng(V)
+    gaps = np.array([9.0, 12.0, 15.0, 17.0, 19.0, 23.0, 30.0])
+    at = np.array([0, 7, V // 3, V // 2, V - 2, V - 1, 11])
+    l = -(np.log(V) + gaps[:, None] + r.uniform(0, 2, (len(gaps), V)))
+    l[np.arange(len(gaps)), at] = 0.0
+    l = l.astype(np.float32 if f32 else np.float16)
+    f, i = dict(dtype=torch.float32, device="cuda"), dict(dtype=torch.int32, device="cuda")
+    R = len(gaps)
+    lp, rank, h = torch.full((R,), float("nan"), **f), torch.full((R,), -7, **i), torch.full((R,), float("nan"), **f)
+    torch.cuda.synchronize()
+    ops.logprobs(torch.from_numpy(l).cuda(), torch.from_numpy(at.astype(np.int32)).cuda(), lp, rank, h, None, None)
+    torch.cuda.synchronize()
+    x = l.astype(np.float64)
+    rest = np.where(x == 0, 0.0, np.exp(x)).sum(1)          # z - 1, without the 1
+    want_lp = -np.log1p(rest)
+    want_h = -want_lp - np.where(x == 0, 0.0, np.exp(x) * x).sum(1) / (1 + rest)
+    assert (rank.cpu().numpy() == 0).all()
+    # relative: an exponent of up to 62 binary orders, 2.8 units of 2^-24 each, 2^y 4, sums and joins (no more than V / 512 steps) 36
+    rel = (2.8 * 62 + 4 + 36 + 3 * (V // 512 + 1)) * 2.0 ** -24
+    for got, want in ((lp, want_lp), (h, want_h)):
+        bad = wrong(got.cpu().numpy(), want, 5 * 2.0 ** -24 + 2 * rel * np.abs(want))
+        assert not bad.any(), (np.argwhere(bad).ravel(), want[bad], got.cpu().numpy()[bad])
