@@ -285,13 +285,18 @@ __global__ void __launch_bounds__(kThreads, min_blocks(sizeof(T), MODE, BYTES, N
     }
 }
 
-// Bound: HBM.  8192 tokens of 40 heads of 128 fp16: 28.6 us (5.9 TB/s; with 256 threads a block 31.8), normalised 33.8; 421 tokens of 28
-// heads of 256, a quarter turned, normalised: 4.8 us.
+// Bound: HBM.  Inputs that change from call to call: 8192 tokens of 40 heads of 128 fp16 as columns of a q/k/v buffer 30.6 us (5.5 TB/s,
+// 0.84 of the copy's rate), apart 29.5, normalised 34.5; 4096 fp32 27.6 (6.1 TB/s); 421 tokens of 28 heads of 256, a quarter turned,
+// normalised: 4.8 us, one wave of dependent latencies.  (Variants are compared, above and below, by calls on the same buffers, part of which
+// the L2 holds: 28.6 us for the first, 31.8 with 256 threads a block.)  Pieces of 4 bytes of fp32 with the weights early keep 48 bytes of a
+// thread in local memory (five blocks an SM).
 
 // The same for any part, alignment and stride: a lane holds sixteen consecutive elements and finds the other element of a pair
 // in shared memory (pitch 17, so that lanes 16 elements apart meet different banks).  Its cos, signed sin and the places of the other
-// elements stay in registers.  Bound: the shared-memory traffic of 8 bytes an element.  4096 tokens of 40 heads of 128 fp16, 42 turned:
-// 25.8 us (k_rope, 44 turned: 18.9); with registers for 4 blocks an SM instead of 5 it was 31.5 us instead of 27.1.
+// elements stay in registers.  Bound: latency, above all of a head's loads, which are asked for only when its turn comes: 4.5 warps a
+// scheduler (96 registers, 27 KB) issue in 46 % of the cycles, shared memory's pipe is busy for 44 %, HBM for 29 %.  4096 tokens of 40
+// heads of 128 fp16, 42 turned, inputs that change: 27.6 us (k_rope, 44 turned: 22.7), 8192: 51.6; with registers for 4 blocks an SM
+// instead of 5 it was 31.5 us instead of 27.1.
 template <typename T, bool NORM>
 __global__ void __launch_bounds__(kThreads, 5) k_rope_any(const RopeParams p, bool wide)
 {

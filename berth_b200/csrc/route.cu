@@ -246,7 +246,8 @@ __device__ __noinline__ bool groups_again(const void* row, unsigned k1, unsigned
 }
 
 // Blocks of an SM that the registers have to allow, and the grid fills once: eight keys a lane, 16384 tokens, 6: 13.8 us, 8: 14.7 us; two
-// keys a lane (64 experts) 8: 7.7 us, 6: 10.3 us.
+// keys a lane (64 experts) 8: 7.7 us, 6: 10.3 us.  Softmax scores of 8 and 16 keys a lane, which were not measured apart, keep 36 to 88
+// bytes of a thread in local memory under these bounds (64 keys: 12 to 32, all orders).
 constexpr int min_blocks(int per) { return per < 8 ? 8 : per == 8 ? 6 : per == 16 ? 4 : 2; }
 
 // One warp per token; lane = P lanes per group, q consecutive experts each.
@@ -265,7 +266,9 @@ constexpr int min_blocks(int per) { return per < 8 ? 8 : per == 8 ? 6 : per == 1
 // softmax, s (2.5 |l - m| + 7) <= 9 S each, S the row's largest, and (2.5 ln E + 6 + PER) |s - s'| for the common 1 / Z, below
 // 2 (28 + PER) S for a pair; the sum with the bias, and the bias less the least, half a step of at most the span each.
 // Bound: instructions, half of them on the half-rate integer pipe, and their latency: 16384 tokens of 256 experts, 8 groups, 8 chosen
-// 13.8 us (17.8 MB would be 2.7), of which 2.5 are a call's least; all of it in 64 bits 57 us.
+// 13.7 us (17.8 MB would be 2.7), of which 2.5 are a call's least; all of it in 64 bits 57 us.  Sigmoid against
+// softmax scores, both under a bias, launches queued ahead: 14.2 and 17.6 us, 8192 tokens of 512 experts 14.8 and 20.1, 16384 of 128 11.6
+// and 13.2.
 template <int PER, bool F32, int ORDER>
 __global__ void __launch_bounds__(128, min_blocks(PER)) k_moe_route(const RouteParams p, bool sigmoid, bool top2, bool wide)
 {
