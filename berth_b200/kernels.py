@@ -359,8 +359,8 @@ class ops:
 
     @staticmethod
     def logprobs(logits, tokens, logprob, rank, entropy, top_idx, top_logprob, vocab: int | None = None, inv_temp: float = 1.0, stream=None) -> None:
-        """Log probabilities under ``softmax(logits * inv_temp)`` in one pass over ``logits`` (fp16 or fp32 ``[rows][>= vocab]``, rows of any
-        stride; ``vocab`` defaults to all columns): ``logprob`` fp32 and ``rank`` int32 ``[rows]`` of ``tokens`` (int32 ``[rows]``),
+        """Log probabilities under ``softmax(logits * inv_temp)`` in one pass over ``logits`` (fp16 or fp32 ``[rows][>= vocab]``, rows that do
+        not overlap; ``vocab`` defaults to all columns): ``logprob`` fp32 and ``rank`` int32 ``[rows]`` of ``tokens`` (int32 ``[rows]``),
         ``entropy`` fp32 ``[rows]``, ``top_idx`` int32 and ``top_logprob`` fp32 ``[rows][n]``, n <= 32, the best alternatives.  Any output
         may be ``None``.  Masks, ties and padding tokens: ``berth_ops_logprobs`` in include/berth_b200.h."""
         (_lib._bind or _lib.bind()).logprobs(logits, tokens, logprob, rank, entropy, top_idx, top_logprob, vocab, inv_temp, _stream(stream))

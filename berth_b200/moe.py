@@ -54,7 +54,7 @@ def _choice(score: str, group_score: str) -> tuple:
 
 def route(logits, selection_bias, topk_idx, topk_w, top_k: int, score: str = "softmax", n_group: int = 1, topk_group: int = 1,
           group_score: str = "max", renormalize: bool = True, scale: float = 1.0, stream=None) -> None:
-    """The experts of every token from its router logits (fp16 or fp32 ``[T][n_experts]``, rows of any stride): ``topk_idx`` int32 and
+    """The experts of every token from its router logits (fp16 or fp32 ``[T][n_experts]``, rows that do not overlap): ``topk_idx`` int32 and
     ``topk_w`` fp32 ``[T][top_k]``.  ``selection_bias`` (fp32 ``[n_experts]`` or ``None``) takes part in the choice only.  The formulas
     and what happens to masked and NaN logits are at ``berth_moe_routing`` in include/berth_b200.h."""
     sc, gs = SCORES.get(score), GROUP_SCORES.get(group_score)

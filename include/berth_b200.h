@@ -262,8 +262,9 @@ int berth_ops_rms_norm_res_in(const void* x, const void* weight, void* y, void* 
  * of a head are contiguous.  y may be x itself (with x's strides); any other overlap of outputs with inputs, or of q's
  * output with k's, is undefined.  The larger stride of an output has to step over all that lies along the smaller one.
  * k may be NULL.  norm of q and of k are independent of each other.
- * positions int32 [n_tokens], any value; inv_freq fp64 [rot_dim / 2]; both device memory.  head_dim up to 512, rot_dim
- * even and at most head_dim.  Rows whose pointers and strides are multiples of 16 bytes take the wide accesses.
+ * positions int32 [n_tokens], any value; inv_freq fp64 [rot_dim / 2]; both device memory.  n_tokens up to 2^30, heads up
+ * to 1024, head_dim up to 512, rot_dim even and at most head_dim.  Strides of the inputs may be 0 (one head or token for
+ * all).  Rows whose pointers and strides are multiples of 16 bytes take the wide accesses.
  * Touches nothing but the tensors; launches on different streams are independent. */
 typedef struct berth_rope_rows {
     const void* x;
@@ -299,7 +300,8 @@ int berth_ops_rope_frequencies(double* inv_freq, int rot_dim, double base, const
  *   top_idx, top_logprob   int32 / fp32 [rows][top_n]: the first top_n tokens of that order and their ln p
  *                (top_n <= 32 and at most vocab; 0: both unused).
  * logits fp16, or fp32 when logits_fp32 != 0; row r starts at element r * row_stride; elements from vocab on are not
- * read.  logprob and rank may be NULL.  inv_temp positive and at most 1e30.
+ * read.  logprob and rank may be NULL.  inv_temp positive and at most 1e30; rows up to 2^26, row_stride at least vocab
+ * (one row: any).  ln p and entropy of a row that is all but certain are off by up to 3e-7.
  * -inf logits are masked tokens: ln p = -inf, nothing added to the entropy.  A row that is masked altogether gives
  * ln p = -inf throughout, entropy 0, and the lowest tokens as alternatives.  A row with a NaN or +inf logit gives NaN for
  * every real number; its whole numbers stay in range (NaN after everything else in the order; rank -1 for a NaN token).
@@ -383,7 +385,8 @@ int berth_moe_router_topk(const void* x, const void* w_router, const float* rout
  * Logits: +inf counts as the largest finite value.  -inf masks an expert: it is chosen only where nothing else is left,
  * and its weight is 0; one masked altogether gives the lowest experts with weights 0.  A masked expert adds nothing to
  * a group's sum.  A NaN logit comes last in the order and makes every weight of its row NaN.  The k indices of a row
- * are always distinct and inside [0, n_experts). */
+ * are always distinct and inside [0, n_experts).  A bias of -inf keeps an expert out as a mask does, but leaves its
+ * weight; one of +inf brings it to the front; a NaN comes last. */
 typedef struct berth_moe_routing {
     int score;                    /* 0 = softmax, 1 = sigmoid */
     int n_group, topk_group;      /* 1, 1: no groups; n_group <= 32 divides n_experts, top_k <= topk_group * n_experts / n_group */
@@ -393,8 +396,8 @@ typedef struct berth_moe_routing {
     const float* selection_bias;  /* fp32 [n_experts], device, or NULL */
 } berth_moe_routing;
 /* The choice alone, from given logits: fp16, or fp32 when logits_fp32 != 0, row t at element t * row_stride; any
- * n_experts up to 1024, top_k up to 32.  topk_idx int32 [T][k] in the order of the choice, topk_w fp32 [T][k].  Needs no
- * workspace. */
+ * n_experts up to 1024, top_k up to 32, T up to 2^30, row_stride at least n_experts (one row: any).  topk_idx int32 [T][k]
+ * in the order of the choice, topk_w fp32 [T][k].  Needs no workspace. */
 int berth_moe_route(const void* logits, int logits_fp32, int64_t row_stride, const float* selection_bias,
                     int32_t* topk_idx, float* topk_w, int T, int n_experts, int top_k, int score, int n_group,
                     int topk_group, int group_score, int renormalize, float scale, void* stream);
