@@ -22,7 +22,7 @@ void stub_let(int on) { let = on; }
 static int wait_for_the_other(void)
 {
     ++inside;
-    for (int i = 0; i < 2000; ++i) {
+    for (int i = 0; i < 10000; ++i) {
         if (let) { --inside; return let > 0 ? 0 : -1; }
         usleep(1000);
     }
